@@ -28,7 +28,10 @@ setup(
             ],
             extra_compile_args={
                 "cxx": ["-O3", "-std=c++17"],
-                "nvcc": ["-O3", "-std=c++17"],
+                # no packed fp32 instructions: some of their forms have
+                # given wrong results on these GPUs
+                "nvcc": ["-O3", "-std=c++17", "-Xclang", "-target-feature",
+                         "-Xclang", "-packed-fp32-ops"],
             },
         )
     ],
