@@ -1499,6 +1499,8 @@ std::tuple<int64_t, int64_t> device_mem_info(int device) {
 
 }  // namespace
 
+void fma_bind_kv8(pybind11::module_& m);  // kv8.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() =
       "MI355X-native sleep/wake actuator (HIP pack/scatter + pinned transfers)";
@@ -1557,6 +1559,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("tensors"), py::arg("offsets"), py::arg("out"),
         py::arg("repeats") = 1);
   m.def("device_mem_info", &device_mem_info, py::arg("device"));
+  fma_bind_kv8(m);
   py::class_<DeviceArena>(m, "DeviceArena")
       .def(py::init<int64_t, int, bool, std::vector<int64_t>>(),
            py::arg("nbytes"), py::arg("device"), py::arg("try_vmm") = false,

@@ -1,0 +1,1137 @@
+// Kernels of a layer's attention side over an 8-bit cache, for gfx950:
+// per-head RMSNorm with the position rotation, the store into the cache,
+// reading it back, and causal attention over it.
+#include "kv8.h"
+
+#include <stdint.h>
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int BLK = FMA_KV8_BLOCK;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kMinAmax = 7.888609052210118e-31f;  // 2^-100
+
+// ---------------------------------------------------------------------------
+// types
+
+struct Bf16 {
+  typedef uint16_t raw;
+  static constexpr uint32_t kInf = 0x7f80, kMaxFinite = 0x7f7f;
+  static __device__ float to_f(uint16_t u) {
+    return __uint_as_float(static_cast<uint32_t>(u) << 16);
+  }
+  static __device__ uint16_t from_f(float f) {
+    return __builtin_bit_cast(uint16_t, static_cast<__bf16>(f));
+  }
+};
+struct Fp16 {
+  typedef uint16_t raw;
+  static constexpr uint32_t kInf = 0x7c00, kMaxFinite = 0x7bff;
+  static __device__ float to_f(uint16_t u) {
+    return static_cast<float>(__builtin_bit_cast(_Float16, u));
+  }
+  static __device__ uint16_t from_f(float f) {
+    return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f));
+  }
+};
+struct Fp32 {
+  typedef float raw;
+  static __device__ float to_f(float f) { return f; }
+  static __device__ float from_f(float f) { return f; }
+};
+
+// Eight values of a row from d0 on; what lies behind hd comes as zero.
+template <typename E>
+__device__ inline void load8(const typename E::raw* row, int d0, int hd,
+                             bool vec, float (&x)[8]) {
+  if (d0 >= hd) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = 0.0f;
+    return;
+  }
+  if constexpr (sizeof(typename E::raw) == 2) {
+    if (vec) {
+      const u16x8 u = *reinterpret_cast<const u16x8*>(row + d0);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = E::to_f(u[j]);
+      return;
+    }
+  } else {
+    if (vec) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(row + d0);
+      const f32x4 b = *reinterpret_cast<const f32x4*>(row + d0 + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = a[j];
+        x[4 + j] = b[j];
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    x[j] = d0 + j < hd ? E::to_f(row[d0 + j]) : 0.0f;
+}
+
+template <typename E>
+__device__ inline void store8(typename E::raw* row, int d0, int hd, bool vec,
+                              const float (&x)[8]) {
+  if (d0 >= hd) return;
+  if constexpr (sizeof(typename E::raw) == 2) {
+    if (vec) {
+      u16x8 u;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = E::from_f(x[j]);
+      *reinterpret_cast<u16x8*>(row + d0) = u;
+      return;
+    }
+  } else {
+    if (vec) {
+      *reinterpret_cast<f32x4*>(row + d0) = f32x4{x[0], x[1], x[2], x[3]};
+      *reinterpret_cast<f32x4*>(row + d0 + 4) = f32x4{x[4], x[5], x[6], x[7]};
+      return;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (d0 + j < hd) row[d0 + j] = E::from_f(x[j]);
+}
+
+// ---------------------------------------------------------------------------
+// Norm and rotation of one head.
+//   y = x * rsqrt(mean(x^2) + eps) * w;  (a, b) -> (a c - b s, a s + b c)
+// A row is held by LPR neighbouring lanes, eight values each, so the mean is
+// log2(LPR) shuffles and pairs (2i, 2i+1) turn inside a lane; the two-halves
+// layout fetches its partner through LDS. All in fp32 with one rounding at
+// the end. The tables are read once for all heads that a row of lanes takes.
+
+template <int LPR>
+__device__ inline float lanes_sum(float x) {
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+
+template <int LPR, bool PAIRS>
+struct Turn {
+  float c[8], s[8];  // of each of the lane's values; s signed in halves
+  float w[8];
+  bool norm;
+  bool bad;  // position outside the table
+
+  // the tables' rows at `pos`; lane holds values d0..d0+7
+  __device__ void at(const FmaRope& r, long long pos, int d0) {
+    bad = r.table > 0 && (pos < 0 || pos >= r.table);
+    const bool on = r.table > 0 && !bad;
+    const float* ct = r.cos + (on ? pos * r.half : 0);
+    const float* st = r.sin + (on ? pos * r.half : 0);
+    if constexpr (PAIRS) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = d0 / 2 + j;
+        const bool in = on && i < r.half;
+        c[j] = in ? ct[i] : 1.0f;
+        s[j] = in ? st[i] : 0.0f;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int d = d0 + j;
+        const bool in = on && d < 2 * r.half;
+        const int i = d < r.half ? d : d - r.half;
+        c[j] = in ? ct[i] : 1.0f;
+        const float sv = in ? st[i] : 0.0f;
+        s[j] = d < r.half ? -sv : sv;
+      }
+    }
+  }
+
+  template <typename E>
+  __device__ void weights(const void* p, int d0, int hd) {
+    norm = p != nullptr;
+    if (norm) {
+      const typename E::raw* q = static_cast<const typename E::raw*>(p);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        w[j] = d0 + j < hd ? E::to_f(q[d0 + j]) : 0.0f;
+    }
+  }
+
+  // scratch: LPR * 8 floats of this row of lanes. The fused multiply-adds
+  // are written out, so that every kernel that runs this gives the same bits.
+  __device__ void run(float (&x)[8], const FmaRope& r, int hd, int d0,
+                      float* scratch) const {
+#pragma clang fp contract(off)
+    if (norm) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+      const float rs =
+          rsqrtf(lanes_sum<LPR>(ss) / static_cast<float>(hd) + r.eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = x[j] * rs * w[j];
+    }
+    if (r.table == 0) return;
+    if constexpr (PAIRS) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (d0 / 2 + j < r.half) {
+          const float a = x[2 * j], b = x[2 * j + 1];
+          x[2 * j] = fmaf(a, c[j], -(b * s[j]));
+          x[2 * j + 1] = fmaf(a, s[j], b * c[j]);
+        }
+      }
+    } else {
+      // value d of the row lies at [d % 8][d / 8]: neighbouring lanes on
+      // neighbouring banks
+      const int li = d0 / 8;
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) scratch[j * LPR + li] = x[j];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int d = d0 + j;
+        if (d < 2 * r.half) {
+          const int p = d < r.half ? d + r.half : d - r.half;
+          x[j] = fmaf(x[j], c[j], scratch[(p & 7) * LPR + (p >> 3)] * s[j]);
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    if (bad) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(0x7fc00000u);
+    }
+  }
+};
+
+__device__ inline long long pos_of(const FmaPos& p, int b, int t) {
+  if (p.p32 == nullptr && p.p64 == nullptr) return p.start + t;
+  const long long i = b * p.sb + (p.per_token ? t * p.st : 0);
+  const long long v = p.p32 != nullptr ? p.p32[i] : p.p64[i];
+  return p.per_token ? v : v + t;
+}
+
+// Heads [h0, h1) of one token, four rows in flight.
+template <typename E, int LPR, bool PAIRS>
+__device__ inline void turn_heads(const Turn<LPR, PAIRS>& turn,
+                                  const FmaRope& r, const FmaRows& in,
+                                  long long base, typename E::raw* out, int h0,
+                                  int h1, int hd, int d0, bool out_vec,
+                                  bool zero, float* scratch) {
+  const typename E::raw* src = static_cast<const typename E::raw*>(in.p) + base;
+  for (int h = h0; h < h1; h += 4) {
+    float x[4][8];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (h + u < h1)
+        load8<E>(src + (h + u) * in.sh, d0, hd, in.vec != 0, x[u]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (h + u < h1) {
+        turn.run(x[u], r, hd, d0, scratch);
+        if (zero) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[u][j] = 0.0f;
+        }
+        store8<E>(out + static_cast<long long>(h + u) * hd, d0, hd, out_vec,
+                  x[u]);
+      }
+    }
+  }
+}
+
+// A row of LPR lanes takes `per` heads of one token.
+template <typename E, int LPR, bool PAIRS>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(
+    FmaRows q, FmaRows k, void* qo, void* ko, int B, int T, int q_heads,
+    int kv_heads, int hd, FmaRope r, FmaPos pos, int per, int q_items,
+    int items) {
+  __shared__ float scratch[256 * 8];
+  const long long unit =
+      static_cast<long long>(blockIdx.x) * (256 / LPR) + threadIdx.x / LPR;
+  const int d0 = (threadIdx.x % LPR) * 8;
+  const long long bt = unit / items;
+  if (bt >= static_cast<long long>(B) * T) return;
+  const int item = static_cast<int>(unit - bt * items);
+  const int b = static_cast<int>(bt / T), t = static_cast<int>(bt - 1LL * b * T);
+  const bool is_q = item < q_items;
+  const int heads = is_q ? q_heads : kv_heads;
+  const int h0 = (is_q ? item : item - q_items) * per;
+  const int h1 = min(h0 + per, heads);
+  const FmaRows in = is_q ? q : k;
+  typename E::raw* out =
+      static_cast<typename E::raw*>(is_q ? qo : ko) + bt * heads * hd;
+  Turn<LPR, PAIRS> turn;
+  turn.at(r, pos_of(pos, b, t), d0);
+  turn.template weights<E>(is_q ? r.qw : r.kw, d0, hd);
+  turn_heads<E, LPR, PAIRS>(turn, r, in, b * in.sb + t * in.st, out, h0, h1,
+                            hd, d0, hd % 8 == 0, false,
+                            scratch + (threadIdx.x / LPR) * LPR * 8);
+}
+
+// ---------------------------------------------------------------------------
+// Cache geometry
+
+// Place of value (token, d) in a block of K: the A operand of
+// v_mfma_f32_16x16x32 for 16 tokens by 32 values has lane 16 g + row hold
+// row's values 8 g .. 8 g + 7; the two halves of the block lie side by side.
+__device__ inline int kidx(int tok, int d) {
+  return (((d >> 5) * 64 + ((d >> 3) & 3) * 16 + (tok & 15)) * 2 +
+          (tok >> 4)) * 8 + (d & 7);
+}
+// Of V: the A operand of V^T, 16 values by 32 tokens. The scores come out of
+// the first product with lane 16 g + row holding tokens 4 g .. 4 g + 3 of
+// each half, so the k index 8 g + 4 half + r of the second product stands
+// for token 16 half + 4 g + r, and the weights need no move between lanes.
+__device__ inline int vidx(int tok, int d) {
+  return (((d >> 5) * 64 + ((tok >> 2) & 3) * 16 + (d & 15)) * 2 +
+          ((d >> 4) & 1)) * 8 + (tok >> 4) * 4 + (tok & 3);
+}
+
+struct Span {
+  int start, count, end;
+};
+__device__ inline Span span_of(const FmaKv8Span& s, int b, int max_seq) {
+  Span o;
+  o.start = s.start != nullptr ? s.start[b] : s.start_i;
+  int n = s.counts != nullptr ? s.counts[b] : s.T;
+  n = min(n, s.T);
+  if (o.start < 0 || o.start > max_seq) n = 0;
+  n = min(n, max_seq - max(o.start, 0));
+  o.count = max(n, 0);
+  if (o.count == 0) o.start = min(max(o.start, 0), max_seq);
+  o.end = o.start + o.count;
+  return o;
+}
+
+// ---------------------------------------------------------------------------
+// Store. One workgroup takes one block of 32 tokens of one kv head: new
+// tokens go through LDS (normed, turned and rounded to 16 bits where asked),
+// a block whose last token is among them is coded, and the new tokens of the
+// last two blocks are also kept raw. Codes are made from the 16-bit values
+// only, so they do not depend on how tokens were spread over calls.
+
+template <typename E>
+__device__ inline bool is_finite16(uint16_t u) {
+  return (u & 0x7fffu) < E::kInf;
+}
+
+// 16 values -> 16 codes. NaN is 0, an infinity the block's largest value.
+template <typename E, bool FP8>
+__device__ inline u32x4 encode16(const uint16_t (&u)[16], float amax,
+                                 float mul) {
+  float x[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float f = E::to_f(u[i]);
+    const uint32_t m = u[i] & 0x7fffu;
+    if (m >= E::kInf) f = m > E::kInf ? 0.0f : copysignf(amax, f);
+    x[i] = f * mul;
+  }
+  u32x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (FP8) {
+      int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
+      w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], w, true);
+      o[i] = static_cast<uint32_t>(w);
+    } else {
+      uint32_t w = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float c = fminf(fmaxf(rintf(x[4 * i + j]), -127.0f), 127.0f);
+        w |= static_cast<uint32_t>(static_cast<int>(c) + 128) << (8 * j);
+      }
+      o[i] = w;
+    }
+  }
+  return o;
+}
+
+// Scale of a block whose largest finite magnitude is amax, and what values
+// are multiplied with before they are rounded. fp8: the smallest power of two
+// that brings amax to 448 or less (scaling is then exact); int8: amax / 127.
+template <bool FP8>
+__device__ inline void scale_of(float amax, float* scale, float* mul) {
+  const float a = fmaxf(amax, kMinAmax);
+  if constexpr (FP8) {
+    const uint32_t bits = __float_as_uint(a);
+    // a = m 2^e: 448 = 1.75 * 2^8
+    const int e = static_cast<int>(bits >> 23) - 127 - 8 +
+                  ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    *scale = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+    *mul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  } else {
+    *scale = a / 127.0f;
+    *mul = 127.0f / a;
+  }
+}
+
+template <typename E, int LPR, bool PAIRS, bool FP8>
+__global__ __launch_bounds__(256) void kv8_append_kernel(
+    FmaKv8Layer c, FmaKv8Span sp, FmaRows q, FmaRows k, FmaRows v, void* qo,
+    int q_heads, FmaRope r, int blocks, int kv_groups, int per, int q_items) {
+  constexpr int MAXD = LPR * 8;
+  constexpr int PITCH = MAXD + 8;
+  __shared__ uint16_t tile[2][BLK][PITCH];
+  __shared__ float scratch[256 * 8];
+  __shared__ uint32_t s_max[2][4];
+  const int tid = threadIdx.x;
+  const int row = tid / LPR, d0 = (tid % LPR) * 8;
+  constexpr int ROWS = 256 / LPR;
+  float* const my_scratch = scratch + row * LPR * 8;
+  const int hd = c.hd;
+
+  if (static_cast<int>(blockIdx.x) >= kv_groups) {
+    // queries
+    const long long unit =
+        static_cast<long long>(blockIdx.x - kv_groups) * ROWS + row;
+    const long long bt = unit / q_items;
+    if (bt >= static_cast<long long>(c.batch) * sp.T) return;
+    const int item = static_cast<int>(unit - bt * q_items);
+    const int b = static_cast<int>(bt / sp.T);
+    const int t = static_cast<int>(bt - 1LL * b * sp.T);
+    const Span s = span_of(sp, b, c.max_seq);
+    Turn<LPR, PAIRS> turn;
+    turn.at(r, s.start + t < c.max_seq ? s.start + t : 0, d0);
+    turn.template weights<E>(r.qw, d0, hd);
+    turn_heads<E, LPR, PAIRS>(
+        turn, r, q, b * q.sb + t * q.st,
+        static_cast<uint16_t*>(qo) + bt * q_heads * hd, item * per,
+        min((item + 1) * per, q_heads), hd, d0, hd % 8 == 0, t >= s.count,
+        my_scratch);
+    return;
+  }
+
+  const int j = blockIdx.x % blocks;
+  const int bh = blockIdx.x / blocks;
+  const int b = bh / c.kv_heads, h = bh - b * c.kv_heads;
+  const Span s = span_of(sp, b, c.max_seq);
+  const int b0 = s.start / BLK, blk = b0 + j;
+  if (s.count == 0 || blk * BLK >= s.end) return;
+  const int open = s.end / BLK;  // the block that is not complete
+  const bool joins = s.start % BLK != 0;
+
+  uint16_t* const tail = static_cast<uint16_t*>(c.tail);
+  auto tail_at = [&](int which, int block) {
+    return tail + which * c.tail_v +
+           (static_cast<long long>(bh) * 2 + (block & 1)) * BLK * c.hdp;
+  };
+
+  // new tokens [lo, hi) of a block, into LDS
+  auto fetch = [&](int block, int lo, int hi) {
+    Turn<LPR, PAIRS> turn;
+    turn.template weights<E>(r.kw, d0, hd);
+    for (int i = lo - block * BLK + row; i < hi - block * BLK; i += ROWS) {
+      const int t = block * BLK + i - s.start;
+      float x[8], y[8];
+      load8<E>(static_cast<const uint16_t*>(k.p) + b * k.sb + t * k.st +
+                   h * k.sh, d0, hd, k.vec != 0, x);
+      load8<E>(static_cast<const uint16_t*>(v.p) + b * v.sb + t * v.st +
+                   h * v.sh, d0, hd, v.vec != 0, y);
+      turn.at(r, block * BLK + i, d0);
+      turn.run(x, r, hd, d0, my_scratch);
+      u16x8 xu, yu;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        xu[e] = d0 + e < hd ? E::from_f(x[e]) : 0;
+        yu[e] = E::from_f(y[e]);
+      }
+      *reinterpret_cast<u16x8*>(&tile[0][i][d0]) = xu;
+      *reinterpret_cast<u16x8*>(&tile[1][i][d0]) = yu;
+    }
+  };
+  // tokens [lo, hi) of a block from LDS to its raw slot
+  auto keep = [&](int block, int lo, int hi) {
+    uint16_t* const kt = tail_at(0, block);
+    uint16_t* const vt = tail_at(1, block);
+    for (int i = lo - block * BLK + row; i < hi - block * BLK; i += ROWS) {
+      if (d0 < c.hdp) {
+        *reinterpret_cast<u16x8*>(kt + kidx(i, d0)) =
+            *reinterpret_cast<const u16x8*>(&tile[0][i][d0]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) vt[vidx(i, d0 + e)] = tile[1][i][d0 + e];
+      }
+    }
+  };
+
+  const int lo = max(s.start, blk * BLK), hi = min(s.end, (blk + 1) * BLK);
+  fetch(blk, lo, hi);
+  const bool complete = hi == (blk + 1) * BLK;
+  if (complete && lo > blk * BLK) {
+    // the block's earlier tokens
+    const uint16_t* const kt = tail_at(0, blk);
+    const uint16_t* const vt = tail_at(1, blk);
+    for (int i = row; i < lo - blk * BLK; i += ROWS) {
+      if (d0 < c.hdp) {
+        *reinterpret_cast<u16x8*>(&tile[0][i][d0]) =
+            *reinterpret_cast<const u16x8*>(kt + kidx(i, d0));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) tile[1][i][d0 + e] = vt[vidx(i, d0 + e)];
+      }
+    }
+  }
+  __syncthreads();
+
+  if (complete) {
+    const int units = c.hdp * 2;  // of 16 values, for each of K and V
+    uint32_t top[2] = {0, 0};
+    for (int i = tid; i < BLK * LPR; i += 256) {
+      const int tok = i / LPR, d = (i % LPR) * 8;
+      if (d < c.hdp) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const u16x8 u = *reinterpret_cast<const u16x8*>(&tile[w][tok][d]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (is_finite16<E>(u[e]))
+              top[w] = max(top[w], static_cast<uint32_t>(u[e] & 0x7fffu));
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      top[0] = max(top[0], static_cast<uint32_t>(__shfl_xor(top[0], o)));
+      top[1] = max(top[1], static_cast<uint32_t>(__shfl_xor(top[1], o)));
+    }
+    if ((tid & 63) == 0) {
+      s_max[0][tid >> 6] = top[0];
+      s_max[1][tid >> 6] = top[1];
+    }
+    __syncthreads();
+    float amax[2], mul[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const uint32_t m = max(max(s_max[w][0], s_max[w][1]),
+                             max(s_max[w][2], s_max[w][3]));
+      amax[w] = E::to_f(static_cast<uint16_t>(m));
+      float scale;
+      scale_of<FP8>(amax[w], &scale, &mul[w]);
+      if (tid == w)
+        c.scales[w * c.scales_v + static_cast<long long>(bh) * c.nblk + blk] =
+            scale;
+    }
+    const long long at =
+        (static_cast<long long>(bh) * c.nblk + blk) * BLK * c.hdp;
+    for (int i = tid; i < 2 * units; i += 256) {
+      const int w = i >= units;
+      const int u = i - w * units;
+      const int l = u & 63, chunk = u >> 6, g = l >> 4, n = l & 15;
+      uint16_t x[16];
+      if (w == 0) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          const u16x8 t8 = *reinterpret_cast<const u16x8*>(
+              &tile[0][16 * a + n][32 * chunk + 8 * g]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[8 * a + e] = t8[e];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          x[e] = tile[1][16 * ((e >> 2) & 1) + 4 * g + (e & 3)]
+                     [32 * chunk + 16 * (e >> 3) + n];
+      }
+      *reinterpret_cast<u32x4*>(c.codes + w * c.codes_v + at + u * 16) =
+          encode16<E, FP8>(x, amax[w], mul[w]);
+    }
+  }
+
+  // A later block of this call may have the slot that this one's earlier
+  // tokens were read from; then it is written here, after that read.
+  if (blk >= open - 1 && !(joins && blk != b0 && (blk & 1) == (b0 & 1)))
+    keep(blk, lo, hi);
+  if (joins && blk == b0) {
+    for (int other = max(open - 1, b0 + 1); other <= open; ++other) {
+      if ((other & 1) == (b0 & 1) && other * BLK < s.end) {
+        const int ohi = min(s.end, (other + 1) * BLK);
+        __syncthreads();
+        fetch(other, other * BLK, ohi);
+        __syncthreads();
+        keep(other, other * BLK, ohi);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Reading back: one workgroup a block of one kv head, through LDS because a
+// token's values do not lie together in V.
+
+template <typename E, bool FP8>
+__global__ __launch_bounds__(256) void kv8_read_kernel(
+    FmaKv8Layer c, const int* start, int start_i, const int* length,
+    int length_i, int n, uint16_t* ko, uint16_t* vo, int blocks) {
+  extern __shared__ uint16_t tile[];  // [BLK][pitch]
+  const int pitch = c.hdp + 8;
+  const int j = blockIdx.x % blocks;
+  const int bh = blockIdx.x / blocks;
+  const int b = bh / c.kv_heads, h = bh - b * c.kv_heads;
+  const int s0 = max(start != nullptr ? start[b] : start_i, 0);
+  int len = length != nullptr ? length[b] : length_i;
+  len = min(max(len, 0), c.max_seq);
+  const int blk = s0 / BLK + j;
+  const int lo = max(s0, blk * BLK);
+  const long long hi_l = min(static_cast<long long>(s0) + n, (blk + 1LL) * BLK);
+  const int hi = static_cast<int>(hi_l);
+  if (hi <= lo) return;
+  const int which = blockIdx.y;
+  uint16_t* const out = which ? vo : ko;
+  const bool any = blk * BLK < len;  // then blk < nblk
+  if (any && blk < len / BLK) {
+    const float scale = c.scales[which * c.scales_v +
+                                 static_cast<long long>(bh) * c.nblk + blk];
+    const unsigned char* const at =
+        c.codes + which * c.codes_v +
+        (static_cast<long long>(bh) * c.nblk + blk) * BLK * c.hdp;
+    for (int u = threadIdx.x; u < c.hdp * 2; u += 256) {
+      const int l = u & 63, chunk = u >> 6, g = l >> 4, m = l & 15;
+      const u32x4 w = *reinterpret_cast<const u32x4*>(at + u * 16);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t byte = (w[e >> 2] >> (8 * (e & 3))) & 255u;
+        float f;
+        if constexpr (FP8)
+          f = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(byte), 0);
+        else
+          f = static_cast<float>(static_cast<int>(byte) - 128);
+        const int tok = which ? 16 * ((e >> 2) & 1) + 4 * g + (e & 3)
+                              : 16 * (e >> 3) + m;
+        const int d = which ? 32 * chunk + 16 * (e >> 3) + m
+                            : 32 * chunk + 8 * g + (e & 7);
+        tile[tok * pitch + d] = E::from_f(f * scale);
+      }
+    }
+  } else if (any) {
+    const uint16_t* const t =
+        static_cast<const uint16_t*>(c.tail) + which * c.tail_v +
+        (static_cast<long long>(bh) * 2 + (blk & 1)) * BLK * c.hdp;
+    for (int i = threadIdx.x; i < BLK * c.hdp; i += 256) {
+      const int tok = i / c.hdp, d = i - tok * c.hdp;
+      tile[tok * pitch + d] = t[which ? vidx(tok, d) : kidx(tok, d)];
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < (hi - lo) * c.hd; i += 256) {
+    const int tok = i / c.hd, d = i - tok * c.hd;
+    const int p = lo + tok;
+    out[((static_cast<long long>(b) * n + (p - s0)) * c.kv_heads + h) * c.hd +
+        d] = p < len ? tile[(p - blk * BLK) * pitch + d] : 0;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Attention. Query rows of one kv head (row = t * group + head) are taken 16
+// at a time; S^T = K Q^T puts a row's scores into lanes 16 g + row, so the
+// softmax is four lanes wide and O^T = V^T P^T takes P as it stands.
+//
+// K and V are made fp16 on the way into the matrix unit: e4m3 and int8 fit
+// exactly. A query row is scaled by a power of two to fit fp16, exactly but
+// for values 2^24 below the row's largest. The weights are rounded to fp16
+// (half a step is 2^-11 of each, against 2^-8 of the bf16 result). A block's
+// K scale multiplies its scores; its V scale relative to a running reference
+// goes into V's conversion (fp8: a power of two, exact) or the weights (int8).
+
+__device__ inline h8 decode8(uint32_t lo, uint32_t hi, float scale, bool fp8) {
+  h2 a, b, cc, d;
+  if (fp8) {
+    a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, false);
+    b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, true);
+    cc = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, false);
+    d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, true);
+  } else {
+    // 0x6400 | u is 1024 + u in fp16; less 1024 + 128 it is the code
+    const h2 off = {static_cast<_Float16>(-1152.0f),
+                    static_cast<_Float16>(-1152.0f)};
+    const uint32_t one = 0x64646464u;
+    a = __builtin_bit_cast(h2, __builtin_amdgcn_perm(one, lo, 0x04010400u)) + off;
+    b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(one, lo, 0x04030402u)) + off;
+    cc = __builtin_bit_cast(h2, __builtin_amdgcn_perm(one, hi, 0x04010400u)) + off;
+    d = __builtin_bit_cast(h2, __builtin_amdgcn_perm(one, hi, 0x04030402u)) + off;
+  }
+  return h8{a[0], a[1], b[0], b[1], cc[0], cc[1], d[0], d[1]};
+}
+
+struct AttnArgs {
+  FmaKv8Layer c;
+  FmaKv8Span sp;
+  FmaRows q;
+  void* out;
+  float* partials;
+  float scale;  // of the scores, times log2(e)
+  int q_heads, group, rows, tiles, splits;
+};
+
+// 16-bit values that are not finite, as finite ones: a weight of zero times
+// them has to be zero.
+template <typename E>
+__device__ inline uint16_t tame(uint16_t u) {
+  const uint32_t m = u & 0x7fffu;
+  if (m < E::kInf) return u;
+  return m > E::kInf ? 0
+                     : static_cast<uint16_t>((u & 0x8000u) | E::kMaxFinite);
+}
+
+template <typename E>
+__device__ inline f32x4 mfma16(u16x8 a, u16x8 b, f32x4 acc) {
+  if constexpr (E::kInf == 0x7f80)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+        __builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), acc, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(
+        __builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), acc, 0, 0, 0);
+}
+
+// One wave's softmax and output state for 16 query rows.
+template <int NS>
+struct RowState {
+  f32x4 o[2 * NS];  // O^T in units of vref: value 16 n + 4 g + reg, row l % 16
+  float m, l;       // running reference and this lane's share of the sum
+  __device__ void clear() {
+#pragma unroll
+    for (int n = 0; n < 2 * NS; ++n) o[n] = f32x4{0, 0, 0, 0};
+    m = -INFINITY;
+    l = 0.0f;
+  }
+  __device__ void times(float f) {
+#pragma unroll
+    for (int n = 0; n < 2 * NS; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[n][r] *= f;
+  }
+  // Scores in units of log2; on return the weights, with the sum advanced.
+  // The reference moves only when a score passes it by 2^8, which fp16
+  // weights and fp32 sums have room for; so the output is rarely rescaled.
+  __device__ void weigh(f32x4 (&x)[2]) {
+    float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                      fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const bool move = top > m + 8.0f || (m == -INFINITY && top > m);
+    if (__any(move)) {
+      const float next = move ? top : m;
+      const float f = move ? exp2f(m - next) : 1.0f;
+      m = next;
+      l *= f;
+      times(f);
+    }
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float sum = 0.0f;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[a][r] = __builtin_amdgcn_exp2f(x[a][r] - ref);
+        sum += x[a][r];
+      }
+    l += sum;
+  }
+};
+
+// Four waves share 16 rows and take the blocks of a split in turn.
+template <int NS, bool FP8, typename E>
+__global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs A) {
+  constexpr int HDP = NS * 32;
+  __shared__ float s_o[4][16][HDP + 4];
+  __shared__ float s_m[4][16], s_l[4][16];
+  const FmaKv8Layer& c = A.c;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g = lane >> 4, n16 = lane & 15;
+  const int split = blockIdx.x % A.splits;
+  const int rest = blockIdx.x / A.splits;
+  const int tile = rest % A.tiles;
+  const int bh = rest / A.tiles;
+  const int b = bh / c.kv_heads, h = bh - b * c.kv_heads;
+  const Span s = span_of(A.sp, b, c.max_seq);
+
+  const int row = tile * 16 + n16;
+  const int t = row / A.group, hq = h * A.group + (row - t * A.group);
+  const bool live = row < A.rows && t < s.count;
+  const int seen = live ? s.start + t + 1 : 0;       // keys of this row
+  const int t_last = min(min(tile * 16 + 15, A.rows - 1) / A.group,
+                         s.count - 1);
+  const int t_first = tile * 16 / A.group;
+  const int most = t_first < s.count ? s.start + t_last + 1 : 0;
+  const int full = s.end / BLK;                      // blocks held as codes
+  const int nb = min(full, (most + BLK - 1) / BLK);
+  const int blk_lo = static_cast<int>(static_cast<long long>(nb) * split / A.splits);
+  const int blk_hi = static_cast<int>(static_cast<long long>(nb) * (split + 1) / A.splits);
+  const bool has_tail = most > full * BLK && split == A.splits - 1;
+
+  RowState<NS> st;
+  st.clear();
+
+  if (blk_lo < blk_hi || has_tail) {
+    // this row's query, as it is and as fp16
+    const uint16_t* const qrow = static_cast<const uint16_t*>(A.q.p) +
+                                 b * A.q.sb + t * A.q.st + hq * A.q.sh;
+    u16x8 qraw[NS];
+    float top = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < NS; ++ks) {
+      const int d = 32 * ks + 8 * g;
+      qraw[ks] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (live && d < c.hd) {
+        if (A.q.vec) {
+          qraw[ks] = *reinterpret_cast<const u16x8*>(qrow + d);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (d + i < c.hd) qraw[ks][i] = qrow[d + i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        top = fmaxf(top, fabsf(E::to_f(qraw[ks][i])));
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    // 2^-e brings the row's largest into [2^9, 2^10)
+    int e = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 9;
+    e = top == 0.0f ? 0 : min(max(e, -100), 100);
+    const float qmul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    const float qscale =
+        A.scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+    h8 qf[NS];
+#pragma unroll
+    for (int ks = 0; ks < NS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        qf[ks][i] = static_cast<_Float16>(E::to_f(qraw[ks][i]) * qmul);
+
+    const unsigned char* const kc =
+        c.codes + static_cast<long long>(bh) * c.nblk * BLK * HDP + lane * 16;
+    const unsigned char* const vc = kc + c.codes_v;
+    const float* const ksc = c.scales + static_cast<long long>(bh) * c.nblk;
+    const float* const vsc = ksc + c.scales_v;
+
+    float vref = 0.0f, vmost = 0.0f;
+    u32x4 kr[NS], vr[NS];
+    auto load = [&](int blk) {
+      const long long at = static_cast<long long>(blk) * BLK * HDP;
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        kr[i] = *reinterpret_cast<const u32x4*>(kc + at + i * 1024);
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        vr[i] = *reinterpret_cast<const u32x4*>(vc + at + i * 1024);
+    };
+    int blk = blk_lo + wave;
+    if (blk < blk_hi) load(blk);
+    for (; blk < blk_hi; blk += 4) {
+      const float kscale = ksc[blk], vscale = vsc[blk];
+      f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+      for (int ks = 0; ks < NS; ++ks) {
+        x[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            decode8(kr[ks][0], kr[ks][1], 1.0f, FP8), qf[ks], x[0], 0, 0, 0);
+        x[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            decode8(kr[ks][2], kr[ks][3], 1.0f, FP8), qf[ks], x[1], 0, 0, 0);
+      }
+      u32x4 v_now[NS];
+#pragma unroll
+      for (int i = 0; i < NS; ++i) v_now[i] = vr[i];
+      if (blk + 4 < blk_hi) load(blk + 4);
+      const float f = kscale * qscale;
+      const int left = seen - blk * BLK - 4 * g;  // tokens of this lane's on
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          x[a][r] = 16 * a + r < left ? x[a][r] * f : -INFINITY;
+      st.weigh(x);
+      // move the reference of V's scales where fp16 has no room for the
+      // ratio; down only as far as fp32 sums cannot overflow
+      if (!(vscale <= vref * 64.0f) ||
+          (vscale < vref * 0.015625f && vscale >= vmost * 5.4e-20f)) {
+        if (vref != 0.0f) st.times(vref / vscale);
+        vref = vscale;
+        vmost = fmaxf(vmost, vscale);
+      }
+      const float ratio = vscale / vref;
+      h8 p;
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          p[4 * a + r] =
+              static_cast<_Float16>(FP8 ? x[a][r] : x[a][r] * ratio);
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        st.o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            decode8(v_now[i][0], v_now[i][1], ratio, FP8), p, st.o[2 * i], 0, 0,
+            0);
+        st.o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            decode8(v_now[i][2], v_now[i][3], ratio, FP8), p, st.o[2 * i + 1],
+            0, 0, 0);
+      }
+    }
+    st.times(vref);
+
+    if (has_tail && wave == 3) {
+      // the block that is not complete, raw. Its weights go in as two 16-bit
+      // parts: a single bf16 would cost as much as the result's rounding.
+      const uint16_t* const kt =
+          static_cast<const uint16_t*>(c.tail) +
+          (static_cast<long long>(bh) * 2 + (full & 1)) * BLK * HDP + lane * 16;
+      const uint16_t* const vt = kt + c.tail_v;
+      f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+      for (int ks = 0; ks < NS; ++ks)
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+          x[a] = mfma16<E>(
+              *reinterpret_cast<const u16x8*>(kt + ks * 1024 + a * 8),
+              qraw[ks], x[a]);
+      const int left = seen - full * BLK - 4 * g;
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          x[a][r] = 16 * a + r < left ? x[a][r] * A.scale : -INFINITY;
+      st.weigh(x);
+      u16x8 hi, lo;
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint16_t u = E::from_f(x[a][r]);
+          hi[4 * a + r] = u;
+          lo[4 * a + r] = E::from_f(x[a][r] - E::to_f(u));
+        }
+      const int held = s.end - full * BLK - 4 * g;
+#pragma unroll
+      for (int n = 0; n < 2 * NS; ++n) {
+        u16x8 vv = *reinterpret_cast<const u16x8*>(vt + (n >> 1) * 1024 +
+                                                   (n & 1) * 8);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          vv[i] = 16 * (i >> 2) + (i & 3) < held ? tame<E>(vv[i]) : 0;
+        st.o[n] = mfma16<E>(vv, hi, st.o[n]);
+        st.o[n] = mfma16<E>(vv, lo, st.o[n]);
+      }
+    }
+  }
+
+  // join the four waves
+  float l = st.l;
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+#pragma unroll
+  for (int n = 0; n < 2 * NS; ++n)
+    *reinterpret_cast<f32x4*>(&s_o[wave][n16][16 * n + 4 * g]) = st.o[n];
+  if (g == 0) {
+    s_m[wave][n16] = st.m;
+    s_l[wave][n16] = l;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * HDP; i += 256) {
+    const int rr = i / HDP, d = i - rr * HDP;
+    const int orow = tile * 16 + rr;
+    if (orow >= A.rows) continue;
+    const float m = fmaxf(fmaxf(s_m[0][rr], s_m[1][rr]),
+                          fmaxf(s_m[2][rr], s_m[3][rr]));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float o = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = exp2f(s_m[w][rr] - ref);
+      o += s_o[w][rr][d] * f;
+      sum += s_l[w][rr] * f;
+    }
+    const int ot = orow / A.group, oh = h * A.group + (orow - ot * A.group);
+    const long long at =
+        (static_cast<long long>(b) * A.sp.T + ot) * A.q_heads + oh;
+    if (A.splits == 1) {
+      if (d < c.hd)
+        static_cast<uint16_t*>(A.out)[at * c.hd + d] =
+            E::from_f(sum == 0.0f ? 0.0f : o / sum);
+    } else {
+      float* const part = A.partials + (at * A.splits + split) * (HDP + 2);
+      part[d] = o;
+      if (d == 0) {
+        part[HDP] = m;
+        part[HDP + 1] = sum;
+      }
+    }
+  }
+}
+
+// Joins the splits of a row, always in the same order.
+template <typename E>
+__global__ __launch_bounds__(256) void kv8_join_kernel(
+    const float* partials, uint16_t* out, long long rows, int splits, int hd,
+    int hdp) {
+  const long long row = blockIdx.x;
+  const float* const p = partials + row * splits * (hdp + 2);
+  float m = -INFINITY;
+  for (int s = 0; s < splits; ++s) m = fmaxf(m, p[s * (hdp + 2) + hdp]);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  for (int d = threadIdx.x; d < hd; d += blockDim.x) {
+    float o = 0.0f, sum = 0.0f;
+    for (int s = 0; s < splits; ++s) {
+      const float f = exp2f(p[s * (hdp + 2) + hdp] - ref);
+      o += p[s * (hdp + 2) + d] * f;
+      sum += p[s * (hdp + 2) + hdp + 1] * f;
+    }
+    out[row * hd + d] = E::from_f(sum == 0.0f ? 0.0f : o / sum);
+  }
+}
+
+int lanes_per_row(int hd) { return hd <= 64 ? 8 : hd <= 128 ? 16 : 32; }
+
+template <typename... P, typename... Given>
+hipError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t lds,
+                  hipStream_t stream, Given... given) {
+  return [&](P... args) {
+    void* list[] = {&args...};
+    return hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid,
+                           dim3(threads), list, lds, stream);
+  }(given...);
+}
+
+}  // namespace
+
+#define FMA_BY_TYPE(type, ...)                                 \
+  if ((type) == 0) { using E = Bf16; __VA_ARGS__; }            \
+  else if ((type) == 1) { using E = Fp16; __VA_ARGS__; }       \
+  else { using E = Fp32; __VA_ARGS__; }
+#define FMA_BY_TYPE16(bf16, ...)                               \
+  if (bf16) { using E = Bf16; __VA_ARGS__; }                   \
+  else { using E = Fp16; __VA_ARGS__; }
+#define FMA_BY_BOOL(cond, NAME, ...)                           \
+  if (cond) { constexpr bool NAME = true; __VA_ARGS__; }       \
+  else { constexpr bool NAME = false; __VA_ARGS__; }
+#define FMA_BY_LANES(hd, ...)                                  \
+  if (lanes_per_row(hd) == 8) { constexpr int LPR = 8; __VA_ARGS__; }          \
+  else if (lanes_per_row(hd) == 16) { constexpr int LPR = 16; __VA_ARGS__; }   \
+  else { constexpr int LPR = 32; __VA_ARGS__; }
+#define FMA_BY_WIDTH(hdp, ...)                                 \
+  switch ((hdp) / 32) {                                        \
+    case 1: { constexpr int NS = 1; __VA_ARGS__; } break;      \
+    case 2: { constexpr int NS = 2; __VA_ARGS__; } break;      \
+    case 3: { constexpr int NS = 3; __VA_ARGS__; } break;      \
+    case 4: { constexpr int NS = 4; __VA_ARGS__; } break;      \
+    case 6: { constexpr int NS = 6; __VA_ARGS__; } break;      \
+    case 8: { constexpr int NS = 8; __VA_ARGS__; } break;      \
+    default: return hipErrorInvalidValue;                      \
+  }
+
+extern "C" hipError_t fma_launch_qk_norm_rope(
+    FmaRows q, FmaRows k, void* qo, void* ko, int B, int T, int q_heads,
+    int kv_heads, int hd, int type, FmaRope rope, FmaPos pos,
+    hipStream_t stream) {
+  const long long tokens = static_cast<long long>(B) * T;
+  if (tokens == 0) return hipSuccess;
+  const int per = tokens * (q_heads + kv_heads) < 8192 ? 1 : 8;
+  const int q_items = (q_heads + per - 1) / per;
+  const int items = q_items + (kv_heads + per - 1) / per;
+  const int rows = 256 / lanes_per_row(hd);
+  const long long grid = (tokens * items + rows - 1) / rows;
+  if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+  FMA_BY_TYPE(type, FMA_BY_LANES(hd, FMA_BY_BOOL(rope.pairs, PAIRS,
+      return launch(qk_norm_rope_kernel<E, LPR, PAIRS>,
+                    dim3(static_cast<unsigned>(grid)), 256, 0, stream, q, k,
+                    qo, ko, B, T, q_heads, kv_heads, hd, rope, pos, per,
+                    q_items, items))));
+}
+
+extern "C" hipError_t fma_launch_kv8_append(FmaKv8Layer c, FmaKv8Span span,
+                                            FmaRows q, FmaRows k, FmaRows v,
+                                            void* qo, int q_heads,
+                                            FmaRope rope, hipStream_t stream) {
+  const long long tokens = static_cast<long long>(c.batch) * span.T;
+  if (tokens == 0) return hipSuccess;
+  int blocks = (span.T + BLK - 2) / BLK + 1;
+  if (span.start == nullptr)
+    blocks = (span.start_i + span.T - 1) / BLK - span.start_i / BLK + 1;
+  const long long kv_groups =
+      static_cast<long long>(c.batch) * c.kv_heads * blocks;
+  const int per = tokens * q_heads < 8192 ? 1 : 8;
+  const int q_items = (q_heads + per - 1) / per;
+  const int rows = 256 / lanes_per_row(c.hd);
+  const long long q_groups =
+      q.p == nullptr ? 0 : (tokens * q_items + rows - 1) / rows;
+  if (kv_groups + q_groups > 0x7fffffffLL) return hipErrorInvalidValue;
+  const unsigned grid = static_cast<unsigned>(kv_groups + q_groups);
+  FMA_BY_TYPE16(c.bf16, FMA_BY_LANES(c.hd, FMA_BY_BOOL(rope.pairs, PAIRS,
+      FMA_BY_BOOL(c.fp8, FP8,
+          return launch(kv8_append_kernel<E, LPR, PAIRS, FP8>, dim3(grid), 256,
+                        0, stream, c, span, q, k, v, qo, q_heads, rope, blocks,
+                        static_cast<int>(kv_groups), per, q_items)))));
+}
+
+extern "C" hipError_t fma_launch_kv8_read(FmaKv8Layer c, const int* start,
+                                          int start_i, const int* length,
+                                          int length_i, int n, void* ko,
+                                          void* vo, hipStream_t stream) {
+  if (n == 0 || c.batch == 0) return hipSuccess;
+  const int blocks = (n + BLK - 2) / BLK + 1;
+  const long long groups = static_cast<long long>(c.batch) * c.kv_heads * blocks;
+  if (groups > 0x7fffffffLL) return hipErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(groups), 2);
+  const size_t lds = static_cast<size_t>(BLK) * (c.hdp + 8) * 2;
+  FMA_BY_TYPE16(c.bf16, FMA_BY_BOOL(c.fp8, FP8,
+      return launch(kv8_read_kernel<E, FP8>, grid, 256, lds, stream, c, start,
+                    start_i, length, length_i, n, static_cast<uint16_t*>(ko),
+                    static_cast<uint16_t*>(vo), blocks)));
+}
+
+extern "C" int fma_kv8_attn_splits(const FmaKv8Layer* c, int T, int q_heads,
+                                   int max_len, int cus) {
+  const long long rows = static_cast<long long>(T) * (q_heads / c->kv_heads);
+  const long long groups =
+      (rows + 15) / 16 * c->batch * c->kv_heads;
+  const int nb = max_len / BLK;
+  // two workgroups a CU, and at least a block for each wave
+  long long splits = groups > 0 ? 2LL * cus / groups : 1;
+  if (splits > nb / 4) splits = nb / 4;
+  return splits < 1 ? 1 : splits > 64 ? 64 : static_cast<int>(splits);
+}
+
+extern "C" hipError_t fma_launch_kv8_attention(FmaKv8Layer c, FmaKv8Span span,
+                                               FmaRows q, void* out,
+                                               int q_heads, float scale,
+                                               float* partials, int splits,
+                                               hipStream_t stream) {
+  if (c.batch == 0 || span.T == 0) return hipSuccess;
+  AttnArgs a;
+  a.c = c;
+  a.sp = span;
+  a.q = q;
+  a.out = out;
+  a.partials = partials;
+  a.scale = scale * kLog2e;
+  a.q_heads = q_heads;
+  a.group = q_heads / c.kv_heads;
+  const long long rows = static_cast<long long>(span.T) * a.group;
+  const long long all = static_cast<long long>(c.batch) * span.T * q_heads;
+  const long long grid =
+      (rows + 15) / 16 * c.batch * c.kv_heads * splits;
+  if (rows > 0x7ffffff0LL || all > 0x7fffffffLL || grid > 0x7fffffffLL)
+    return hipErrorInvalidValue;
+  a.rows = static_cast<int>(rows);
+  a.tiles = static_cast<int>((rows + 15) / 16);
+  a.splits = splits;
+  hipError_t err = hipSuccess;
+  FMA_BY_TYPE16(c.bf16, FMA_BY_BOOL(c.fp8, FP8, FMA_BY_WIDTH(c.hdp,
+      err = launch(kv8_attn_kernel<NS, FP8, E>,
+                   dim3(static_cast<unsigned>(grid)), 256, 0, stream, a))));
+  if (err != hipSuccess || splits == 1) return err;
+  const int threads = c.hd <= 64 ? 64 : c.hd <= 128 ? 128 : 256;
+  FMA_BY_TYPE16(c.bf16,
+      return launch(kv8_join_kernel<E>, dim3(static_cast<unsigned>(all)),
+                    threads, 0, stream, partials, static_cast<uint16_t*>(out),
+                    all, splits, c.hd, c.hdp));
+}

@@ -66,6 +66,105 @@ def fast_rope1(x: torch.Tensor, cos_row: torch.Tensor, sin_row: torch.Tensor
     return out.view(B, T, heads, hd).to(x.dtype)
 
 
+def _check_rope(q, k, cos, sin, q_norm, k_norm) -> None:
+    hd = q.shape[-1]
+    if cos.dim() != 2 or cos.shape != sin.shape \
+            or cos.dtype != torch.float32 or sin.dtype != torch.float32 \
+            or not (cos.is_contiguous() and sin.is_contiguous()) \
+            or cos.device != q.device or sin.device != q.device:
+        raise ValueError("cos/sin must be contiguous fp32 [S, rot/2] on "
+                         f"{q.device}")
+    if not 1 <= cos.shape[1] <= hd // 2 or cos.shape[0] < 1:
+        raise ValueError(f"tables of {list(cos.shape)} cannot rotate heads "
+                         f"of {hd}")
+    for w in (q_norm, k_norm):
+        if w is not None and (w.shape != (hd,) or w.dtype != q.dtype
+                              or w.device != q.device
+                              or not w.is_contiguous()):
+            raise ValueError(f"norm weights must be contiguous {q.dtype} "
+                             f"[{hd}] on {q.device}")
+
+
+def rope_rows(x, w, cos, sin, pos, eps: float, interleaved: bool):
+    """The plain form of :func:`fast_qk_norm_rope` for one of its tensors;
+    pos [B, T] within the tables."""
+    y = x.float()
+    if w is not None:
+        y = y * torch.rsqrt(y.pow(2).mean(-1, keepdim=True) + eps) * w.float()
+    c, s = cos[pos].unsqueeze(2), sin[pos].unsqueeze(2)
+    n = cos.shape[1]
+    if interleaved:
+        a, b = y[..., 0:2 * n:2], y[..., 1:2 * n:2]
+        r = torch.stack((a * c - b * s, a * s + b * c), -1).flatten(-2)
+    else:
+        a, b = y[..., :n], y[..., n:2 * n]
+        r = torch.cat((a * c - b * s, a * s + b * c), -1)
+    return torch.cat((r, y[..., 2 * n:]), -1).to(x.dtype)
+
+
+def fast_qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor,
+                      sin: torch.Tensor, pos, q_norm=None, k_norm=None,
+                      eps: float = 1e-6, interleaved: bool = True):
+    """RMSNorm of each query and key head over its head_dim, then the position
+    rotation, in one pass: fp32 inside, rounded once. Returns new (q, k).
+
+    q [B, T, qH, hd], k [B, T, kvH, hd] in bf16, fp16 or fp32, any strides
+    but a contiguous last dimension (views of a fused projection need no
+    copy). q_norm / k_norm [hd]: gains, None leaves that norm out. cos / sin
+    fp32 [S, rot/2]: the first rot of hd values turn, the rest passes; a
+    factor for long contexts belongs into the tables. Pairs are (2i, 2i+1),
+    or with interleaved=False (i, i + rot/2). pos: the first token's position
+    as a number, or int32 / int64 [B] of first positions, or [B, T] of every
+    token's. A position outside the tables is refused where the host knows
+    it; one that only the GPU knows gives NaN.
+
+    One launch on the GPU for any T; torch operations on the CPU."""
+    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] \
+            or q.shape[3] != k.shape[3] or q.shape[2] < 1 or k.shape[2] < 1:
+        raise ValueError(f"q {list(q.shape)} and k {list(k.shape)} must be "
+                         "[B, T, heads, head_dim] alike but for the heads")
+    if q.dtype != k.dtype or q.device != k.device or q.dtype not in (
+            torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError("q and k must both be bf16, fp16 or fp32 on one "
+                         "device")
+    B, T, _, hd = q.shape
+    if not 2 <= hd <= 256:
+        raise ValueError(f"head_dim must be 2..256, got {hd}")
+    if (q.requires_grad or k.requires_grad) and torch.is_grad_enabled():
+        raise ValueError("q or k requires a gradient; this has no backward "
+                         "pass")
+    _check_rope(q, k, cos, sin, q_norm, k_norm)
+    given = isinstance(pos, torch.Tensor)
+    if given:
+        if pos.dtype not in (torch.int32, torch.int64) \
+                or pos.device != q.device \
+                or pos.shape not in ((B,), (B, T)):
+            raise ValueError(f"pos must be int32 or int64 [{B}] or "
+                             f"[{B}, {T}] on {q.device}")
+    elif pos < 0 or pos + T > cos.shape[0]:
+        raise ValueError(f"positions [{pos}, {pos + T}) lie outside the "
+                         f"tables' {cos.shape[0]}")
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    if k.stride(3) != 1:
+        k = k.contiguous()
+    if q.is_cuda:
+        return actuation.require_native().qk_norm_rope(
+            q, k, cos, sin, pos if given else None, 0 if given else pos,
+            q_norm, k_norm, float(eps), interleaved)
+    if not given:
+        pos = torch.full((B,), pos, dtype=torch.long)
+    if pos.dim() == 1:
+        pos = pos.long()[:, None] + torch.arange(T)
+    pos = pos.long()
+    out = (pos < 0) | (pos >= cos.shape[0])
+    pos = pos.clamp(0, cos.shape[0] - 1)
+    nan = torch.full((), float("nan"), dtype=q.dtype)
+    return tuple(torch.where(out[:, :, None, None], nan, rope_rows(
+        x, w, cos, sin, pos, eps, interleaved))
+        for x, w in ((q, q_norm), (k, k_norm)))
+
+
 def fast_rope_qkv_store(q, k, v, kcache, vcache, cos_tab, sin_tab,
                         pos=None, pos_dev=None) -> bool:
     """RoPE(q in place) + RoPE(k)->cache + v->cache in ONE launch

@@ -25,6 +25,8 @@ setup(
             sources=[
                 "fma_amd/csrc/actuator.cpp",
                 "fma_amd/csrc/kernels.hip",
+                "fma_amd/csrc/kv8.cpp",
+                "fma_amd/csrc/kv8.hip",
             ],
             extra_compile_args={
                 "cxx": ["-O3", "-std=c++17"],

@@ -1,0 +1,255 @@
+"""The 8-bit cache and norm + rotation on the CPU: formulas, bookkeeping and
+refusals."""
+
+import pytest
+import torch
+
+from fma_amd.ops.decode_ops import fast_qk_norm_rope
+from fma_amd.ops.kv8 import (KV8Cache, kv8_append, kv8_attention, kv8_read,
+                             qk_norm_rope_kv8)
+from tests import kv8_oracle as oracle
+
+
+def make(fmt="fp8", dtype=torch.bfloat16, B=1, S=100, H=2, hd=16, layers=1):
+    return KV8Cache(layers, B, S, H, hd, fmt=fmt, dtype=dtype)
+
+
+def value(x, dtype):
+    """A held value as kv8_read gives it: the product of code and scale is
+    exact in 64 bits, so this is its fp32 rounding and then the type's."""
+    return x.float().to(dtype)
+
+
+def kv(T, B=1, H=2, hd=16, dtype=torch.bfloat16, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    k = torch.randn(B, T, H, hd, generator=g) * 3
+    v = torch.randn(B, T, H, hd, generator=g)
+    return k.to(dtype), v.to(dtype)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_read_gives_what_the_definition_says(fmt, dtype):
+    c = make(fmt, dtype, hd=20)
+    k, v = kv(75, hd=20, dtype=dtype)
+    kv8_append(c, 0, k, v, 0)
+    rk, rv = kv8_read(c, 0, 0, 80, 75)
+    assert torch.equal(rk[0, :75], value(oracle.held(k[0], fmt), dtype))
+    assert torch.equal(rv[0, :75], value(oracle.held(v[0], fmt), dtype))
+    assert not rk[0, 75:].any() and not rv[0, 75:].any()
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+def test_result_does_not_depend_on_how_tokens_arrive(fmt):
+    k, v = kv(97)
+    whole, parts = make(fmt), make(fmt)
+    kv8_append(whole, 0, k, v, 0)
+    at = 0
+    for n in (1, 30, 1, 5, 40, 3, 17):
+        kv8_append(parts, 0, k[:, at:at + n], v[:, at:at + n], at)
+        at += n
+    for a, b in zip(kv8_read(whole, 0, 0, 97, 97),
+                    kv8_read(parts, 0, 0, 97, 97)):
+        assert torch.equal(a, b)
+
+
+def test_not_finite_values():
+    c = make()
+    k, v = kv(40)
+    k[0, 3, 0, 1], k[0, 4, 1, 2] = float("nan"), float("inf")
+    v[0, 5, 0, 0] = float("-inf")
+    kv8_append(c, 0, k, v, 0)
+    rk, rv = kv8_read(c, 0, 0, 32, 40)
+    assert rk[0, 3, 0, 1] == 0
+    assert torch.equal(rk[0], value(oracle.held(k[0, :32], "fp8"), k.dtype))
+    assert torch.equal(rv[0], value(oracle.held(v[0, :32], "fp8"), v.dtype))
+
+
+def test_zero_block_and_tiny_values():
+    for fmt in ("fp8", "int8"):
+        c = make(fmt)
+        k = torch.zeros(1, 32, 2, 16, dtype=torch.bfloat16)
+        v = torch.full_like(k, 2.0 ** -110)
+        kv8_append(c, 0, k, v, 0)
+        rk, rv = kv8_read(c, 0, 0, 32, 32)
+        assert not rk.any()
+        assert torch.equal(rv[0], value(oracle.held(v[0], fmt), v.dtype))
+
+
+def test_going_back_after_a_rejected_draft():
+    k, v = kv(80)
+    c = make()
+    kv8_append(c, 0, k[:, :62], v[:, :62], 0)
+    junk_k, junk_v = kv(5, seed=9)
+    kv8_append(c, 0, junk_k, junk_v, 62)     # completes a block, with junk
+    kv8_append(c, 0, k[:, 62:80], v[:, 62:80], 62)
+    ref = make()
+    kv8_append(ref, 0, k, v, 0)
+    for a, b in zip(kv8_read(c, 0, 0, 80, 80), kv8_read(ref, 0, 0, 80, 80)):
+        assert torch.equal(a, b)
+
+
+def test_later_block_in_the_slot_of_the_first():
+    """One call that reads a block's earlier tokens and ends in a block that
+    is held in the same slot."""
+    for end in (70, 96, 97, 130):
+        k, v = kv(end)
+        c, ref = make(S=200), make(S=200)
+        kv8_append(c, 0, k[:, :5], v[:, :5], 0)
+        kv8_append(c, 0, k[:, 5:], v[:, 5:], 5)
+        kv8_append(ref, 0, k, v, 0)
+        for a, b in zip(kv8_read(c, 0, 0, end, end),
+                        kv8_read(ref, 0, 0, end, end)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("T", [1, 3, 40])
+def test_attention_matches_the_oracle(fmt, T):
+    k, v = kv(90)
+    c = make(fmt)
+    kv8_append(c, 0, k, v, 0)
+    q = torch.randn(1, T, 6, 16, generator=torch.Generator().manual_seed(3)) \
+        .bfloat16()
+    out = kv8_attention(q, c, 0, 90 - T)
+    want, bound = oracle.attention(q[0], oracle.held(k[0], fmt),
+                                   oracle.held(v[0], fmt), 90 - T, 0.25)
+    oracle.check(out[0], want, bound, q.dtype)
+
+
+def test_ragged_batch():
+    k, v = kv(50, B=3)
+    c = make(B=3)
+    start = torch.tensor([0, 0, 0], dtype=torch.int32)
+    counts = torch.tensor([50, 0, 33], dtype=torch.int32)
+    kv8_append(c, 0, k, v, start, counts)
+    q = torch.randn(3, 50, 2, 16).bfloat16()
+    out = kv8_attention(q, c, 0, start, counts)
+    assert not out[1].any() and not out[2, 33:].any()
+    for b, n in ((0, 50), (2, 33)):
+        want, bound = oracle.attention(
+            q[b, :n], oracle.held(k[b, :n], "fp8"),
+            oracle.held(v[b, :n], "fp8"), 0, 0.25)
+        oracle.check(out[b, :n], want, bound, q.dtype)
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("rot,norm", [(16, True), (10, True), (6, False)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16,
+                                   torch.float32])
+def test_norm_rope_matches_the_oracle(interleaved, rot, norm, dtype):
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn(2, 5, 4, 16, generator=g).to(dtype)
+    k = torch.randn(2, 5, 2, 16, generator=g).to(dtype)
+    cos, sin = oracle.tables(50, rot, factor=1.2)
+    w = [torch.rand(16, generator=g).to(dtype) if norm else None
+         for _ in range(2)]
+    pos = torch.randint(0, 50, (2, 5), generator=g)
+    got = fast_qk_norm_rope(q, k, cos, sin, pos, *w, interleaved=interleaved)
+    for x, y, g_ in zip((q, k), got, w):
+        want, bound = oracle.norm_rope(x, g_, cos, sin, pos, 1e-6,
+                                       interleaved)
+        oracle.check(y, want, bound, dtype)
+
+
+def test_norm_rope_position_forms_and_outside():
+    q, k = torch.randn(2, 3, 2, 8), torch.randn(2, 3, 1, 8)
+    cos, sin = oracle.tables(10, 8)
+    a = fast_qk_norm_rope(q, k, cos, sin, 4)
+    b = fast_qk_norm_rope(q, k, cos, sin, torch.tensor([4, 4]))
+    c = fast_qk_norm_rope(q, k, cos, sin,
+                          torch.tensor([[4, 5, 6]] * 2, dtype=torch.int32))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], c[1])
+    d = fast_qk_norm_rope(q, k, cos, sin, torch.tensor([8, -1]))
+    assert torch.isnan(d[0][0, 2]).all() and torch.isnan(d[1][1, 0]).all()
+    assert torch.isfinite(d[0][0, :2]).all()
+
+
+def test_one_call_is_the_two_calls():
+    q = torch.randn(1, 40, 4, 16).bfloat16()
+    k, v = kv(40)
+    cos, sin = oracle.tables(100, 16)
+    w = torch.rand(16).bfloat16()
+    a, b = make(), make()
+    qa = qk_norm_rope_kv8(a, 0, q, k, v, cos, sin, 0, w, w)
+    qb, kb = fast_qk_norm_rope(q, k, cos, sin, 0, w, w)
+    kv8_append(b, 0, kb, v, 0)
+    assert torch.equal(qa, qb)
+    for x, y in zip(kv8_read(a, 0, 0, 40, 40), kv8_read(b, 0, 0, 40, 40)):
+        assert torch.equal(x, y)
+
+
+def test_refusals_of_the_cache():
+    for bad in (dict(fmt="int4"), dict(dtype=torch.float32), dict(hd=257),
+                dict(hd=0), dict(S=0), dict(B=0)):
+        with pytest.raises(ValueError):
+            make(**bad)
+    c = make()
+    k, v = kv(10)
+    for args in ((1, k, v, 0), (-1, k, v, 0), (0, k[..., :8], v, 0),
+                 (0, k.float(), v, 0), (0, k[:, :, :1], v, 0),
+                 (0, k, v[:, :5], 0), (0, k, v, -1), (0, k, v, 91),
+                 (0, k, v, 5), (0, k[0], v, 0),
+                 (0, k, v, torch.tensor([0])),
+                 (0, k, v, torch.tensor([0, 0], dtype=torch.int32)),
+                 (0, k, v, 0, torch.tensor([3]))):
+        with pytest.raises(ValueError):
+            kv8_append(c, *args)
+    with pytest.raises(ValueError):
+        kv8_append(c, 0, k.float().requires_grad_().bfloat16(), v, 0)
+    kv8_append(c, 0, k, v, 0)
+    q = torch.randn(1, 1, 2, 16).bfloat16()
+    for args in ((q, c, 0, 10), (q, c, 0, 100), (q, c, 3, 9),
+                 (q.float(), c, 0, 9), (q[:, :, :1], c, 0, 9)):
+        with pytest.raises(ValueError):
+            kv8_attention(*args)
+    for args in ((0, 0, -1, 5), (0, 101, 1, 5), (0, 0, 1, 101)):
+        with pytest.raises(ValueError):
+            kv8_read(c, *args)
+    c.free()
+    with pytest.raises(ValueError):
+        kv8_append(c, 0, k, v, 0)
+
+
+def test_refuses_to_build_on_values_it_no_longer_holds():
+    c = make(S=300)
+    k, v = kv(200)
+    kv8_append(c, 0, k, v, 0)                 # blocks 5 and 6 are raw
+    one = kv(1)
+    for start in (159, 100, 33):
+        with pytest.raises(ValueError, match="raw values"):
+            kv8_append(c, 0, *one, start)
+    with pytest.raises(ValueError, match="hole"):
+        kv8_append(c, 0, *one, 201)
+    kv8_append(c, 0, *one, 161)               # one block back
+    with pytest.raises(ValueError, match="holds 162"):
+        kv8_attention(torch.zeros(1, 1, 2, 16).bfloat16(), c, 0, 162)
+    with pytest.raises(ValueError, match="raw values"):
+        kv8_append(c, 0, *one, 159)
+    kv8_append(c, 0, *one, 128)               # a block's first token
+    kv8_append(c, 0, *one, 129)
+    with pytest.raises(ValueError, match="raw values"):
+        kv8_append(c, 0, *one, 127)
+    c.reset()
+    kv8_append(c, 0, *one, 0)
+
+
+def test_refusals_of_norm_rope():
+    q, k = torch.randn(1, 2, 2, 8), torch.randn(1, 2, 1, 8)
+    cos, sin = oracle.tables(10, 8)
+    w = torch.ones(8)
+    for args in ((q[0], k[0], cos, sin, 0), (q, k[:, :1], cos, sin, 0),
+                 (q, k.half(), cos, sin, 0), (q, k, cos, sin[:5], 0),
+                 (q, k, cos.half(), sin.half(), 0),
+                 (q, k, *oracle.tables(10, 10), 0), (q, k, cos, sin, 9),
+                 (q, k, cos, sin, -1), (q, k, cos, sin, torch.zeros(2).long()),
+                 (q, k, cos, sin, torch.zeros(1)),
+                 (q, k, cos, sin, 0, w[:4]), (q, k, cos, sin, 0, w.half()),
+                 (q.requires_grad_(), k, cos, sin, 0)):
+        with pytest.raises(ValueError):
+            fast_qk_norm_rope(*args)
+    c = make(hd=8)
+    kk, v = kv(2, hd=8)
+    with pytest.raises(ValueError, match="tables"):
+        qk_norm_rope_kv8(c, 0, torch.zeros(1, 2, 2, 8).bfloat16(), kk, v,
+                         cos, sin, 0)
