@@ -29,6 +29,7 @@ from fma_amd.ops.decode_ops import (available as _fused_available,
                                     fast_rope_qkv_store,
                                     fast_rmsnorm, fast_rope1,
                                     fast_silu_mul)
+from fma_amd.ops.kv8 import kv8_attention, qk_norm_rope_kv8
 from fma_amd.ops.linear import (fast_linear, fast_linear_multi,
                                 fast_linear_residual)
 
@@ -49,11 +50,15 @@ class StaticDecoder:
     """Single-token decode with static shapes over a private KV cache."""
 
     @staticmethod
-    def supported(cfg) -> bool:
+    def supported(cfg, kv_cache_dtype: str = "auto") -> bool:
         # MoE routing is data-dependent per token: un-capturable;
-        # qk_norm (qwen3) is outside the fused qkv+rope capture set
-        return (cfg.vocab_size <= GRAPH_SAFE_VOCAB and not cfg.num_experts
-                and not cfg.qk_norm)
+        # qk_norm (qwen3) is outside the fused qkv+rope capture set, but
+        # inside the 8-bit cache's one-launch norm + rope + store
+        if cfg.vocab_size > GRAPH_SAFE_VOCAB or cfg.num_experts:
+            return False
+        if kv_cache_dtype != "auto":
+            return cfg.hidden_act == "silu" and not cfg.embed_scale
+        return not cfg.qk_norm
 
     def __init__(self, model: LlamaModel, batch: int, max_seq: int):
         assert model.tp_size == 1, "graphed decode is single-rank for now"
@@ -64,9 +69,16 @@ class StaticDecoder:
         dev = model.device
         cfg = self.cfg
         kv_heads = cfg.num_kv_heads
-        self.cache = torch.zeros(
-            (cfg.num_layers, 2, batch, max_seq, kv_heads, cfg.head_dim),
-            dtype=cfg.dtype, device=dev)
+        self.kv8 = None
+        if model.kv_cache_dtype != "auto":
+            self.kv8 = model.new_cache(batch, max_seq)
+            self.start_i32 = torch.zeros((batch,), dtype=torch.int32,
+                                         device=dev)
+            self.cache = None
+        else:
+            self.cache = torch.zeros(
+                (cfg.num_layers, 2, batch, max_seq, kv_heads, cfg.head_dim),
+                dtype=cfg.dtype, device=dev)
         self.input_tok = torch.zeros((batch, 1), dtype=torch.long, device=dev)
         self.pos = torch.zeros((), dtype=torch.long, device=dev)
         self.positions = torch.arange(max_seq, device=dev)
@@ -104,7 +116,9 @@ class StaticDecoder:
         fused_attn = (B == 1 and x.is_cuda and x.dtype == torch.bfloat16
                       and hd % 64 == 0 and hd <= 256
                       and q_heads % kv_heads == 0 and _fused_available())
-        if fused_attn:
+        if self.kv8 is not None:
+            self.start_i32.copy_(self.pos.to(torch.int32).expand(B))
+        elif fused_attn:
             self.t_i32.copy_((self.pos + 1).to(torch.int32))
         self.pos_i32.copy_(self.pos.to(torch.int32).view(1))
         # additive mask over the full window: position j attends iff j <= pos
@@ -125,8 +139,14 @@ class StaticDecoder:
             q = q.view(B, 1, q_heads, hd)
             k = k.view(B, 1, kv_heads, hd)
             v = v.view(B, 1, kv_heads, hd)
-            stored = False
-            if B == 1 and q.is_cuda and q.dtype == torch.bfloat16:
+            stored = self.kv8 is not None
+            if stored:
+                # the position is read on the device at replay time
+                q = qk_norm_rope_kv8(
+                    self.kv8, li, q, k, v, m.rope_cos, m.rope_sin,
+                    self.start_i32, P.get(p + "q_norm.weight"),
+                    P.get(p + "k_norm.weight"), eps=cfg.norm_eps)
+            elif B == 1 and q.is_cuda and q.dtype == torch.bfloat16:
                 # one graph-safe launch: RoPE(q) + RoPE(k)->cache +
                 # v->cache, position read from the device scalar at
                 # replay time
@@ -143,7 +163,10 @@ class StaticDecoder:
                 # static cache write at pos
                 self.cache[li, 0].index_copy_(1, self.pos.view(1), k)
                 self.cache[li, 1].index_copy_(1, self.pos.view(1), v)
-            if fused_attn:
+            if self.kv8 is not None:
+                att = kv8_attention(q, self.kv8, li, self.start_i32) \
+                    .view(B, 1, q_heads * hd)
+            elif fused_attn:
                 from fma_amd.ops import actuation
                 att = actuation._C.attn_decode_bf16_graph(
                     q.reshape(q_heads, hd).contiguous(),
@@ -198,14 +221,19 @@ class StaticDecoder:
                 self.step_()
         torch.cuda.current_stream().wait_stream(s)
         # reset state disturbed by warmup
-        self.pos.zero_()
-        self.cache.zero_()
+        self._clear()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             self.step_()
         self.graph = g
+        self._clear()
+
+    def _clear(self) -> None:
         self.pos.zero_()
-        self.cache.zero_()
+        if self.kv8 is not None:
+            self.kv8.reset()
+        else:
+            self.cache.zero_()
 
     @torch.no_grad()
     def prefill(self, prompt: torch.Tensor) -> None:
@@ -215,11 +243,11 @@ class StaticDecoder:
 
         B, T = prompt.shape
         assert B == self.batch and T < self.max_seq
-        self.pos.zero_()
-        self.cache.zero_()
+        self._clear()
         self.out_tokens.zero_()
         if T > 1:
-            cache_view = SimpleNamespace(data=self.cache)
+            cache_view = self.kv8 if self.kv8 is not None \
+                else SimpleNamespace(data=self.cache)
             logits = self.model.forward(prompt, cache_view, 0)
             nxt = logits[:, -1].argmax(-1, keepdim=True)
             self.pos.fill_(T)

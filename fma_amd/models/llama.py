@@ -30,6 +30,8 @@ import torch.nn.functional as F
 from fma_amd.ops.decode_ops import (fast_attn_decode, fast_attn_prefill,
                                     fast_rmsnorm, fast_rope1,
                                     fast_rope_qkv_store, fast_silu_mul)
+from fma_amd.ops.kv8 import (FORMATS, KV8Cache, kv8_attention,
+                             qk_norm_rope_kv8)
 from fma_amd.ops.linear import (fast_linear, fast_linear_multi,
                                 fast_linear_residual)
 
@@ -393,19 +395,46 @@ class KVCache:
         self.data = None  # type: ignore[assignment]
 
 
+def check_kv_cache_dtype(cfg: LlamaConfig, kv_cache_dtype: str) -> str:
+    """"auto" (the model's type), or a format of :class:`KV8Cache` that can
+    hold this model's keys and values."""
+    if kv_cache_dtype == "auto":
+        return kv_cache_dtype
+    if kv_cache_dtype not in FORMATS:
+        raise ValueError(f"unknown kv_cache_dtype {kv_cache_dtype!r}: "
+                         f"auto or one of {FORMATS}")
+    if cfg.dtype not in (torch.bfloat16, torch.float16) or cfg.head_dim > 256:
+        raise ValueError(f"an 8-bit cache needs a 16-bit model and heads of "
+                         f"at most 256, not {cfg.dtype} and {cfg.head_dim}")
+    return kv_cache_dtype
+
+
 class LlamaModel:
     """Functional Llama over a dict of (arena-view) tensors."""
 
     def __init__(self, cfg: LlamaConfig, params: Dict[str, torch.Tensor],
                  device, tp_rank: int = 0, tp_size: int = 1,
-                 tp_group: Optional[object] = None):
+                 tp_group: Optional[object] = None,
+                 kv_cache_dtype: str = "auto"):
         self.cfg = cfg
+        self.kv_cache_dtype = check_kv_cache_dtype(cfg, kv_cache_dtype)
         self.params = params
         self.device = device
         self.tp_rank = tp_rank
         self.tp_size = tp_size
         self.tp_group = tp_group
         self.rope_cos, self.rope_sin = precompute_rope(cfg, device)
+
+    def new_cache(self, batch: int, max_seq: Optional[int] = None):
+        """A cache of this model's ``kv_cache_dtype`` for :meth:`forward`."""
+        if self.kv_cache_dtype == "auto":
+            return KVCache(self.cfg, batch, self.device, self.tp_size,
+                           max_seq)
+        return KV8Cache(self.cfg.num_layers, batch,
+                        max_seq or self.cfg.max_seq_len,
+                        max(self.cfg.num_kv_heads // self.tp_size, 1),
+                        self.cfg.head_dim, fmt=self.kv_cache_dtype,
+                        dtype=self.cfg.dtype, device=self.device)
 
     def rebind(self, params: Dict[str, torch.Tensor]) -> None:
         """Swap in fresh views after a non-VMM wake changed the arena base."""
@@ -507,7 +536,8 @@ class LlamaModel:
         return x + self._maybe_all_reduce(out)
 
     @torch.no_grad()
-    def forward(self, tokens: torch.Tensor, cache: Optional[KVCache] = None,
+    def forward(self, tokens: torch.Tensor,
+                cache: "KVCache | KV8Cache | None" = None,
                 start_pos: int = 0) -> torch.Tensor:
         """tokens [B, T] -> logits [B, T, vocab]."""
         cfg = self.cfg
@@ -551,11 +581,22 @@ class LlamaModel:
             q = q.view(B, T, q_heads, hd)
             k = k.view(B, T, kv_heads, hd)
             v = v.view(B, T, kv_heads, hd)
-            if cfg.qk_norm:
+            att = None
+            kv8 = isinstance(cache, KV8Cache)
+            if kv8:
+                # norms, rotation and store in one launch; attention reads
+                # the codes
+                q = qk_norm_rope_kv8(
+                    cache, li, q, k, v, self.rope_cos, self.rope_sin,
+                    start_pos, P.get(p + "q_norm.weight"),
+                    P.get(p + "k_norm.weight"), eps=cfg.norm_eps)
+                att = kv8_attention(q, cache, li, start_pos) \
+                    .view(B, T, q_heads * hd)
+            elif cfg.qk_norm:
                 q = rmsnorm(q, P[p + "q_norm.weight"], cfg.norm_eps)
                 k = rmsnorm(k, P[p + "k_norm.weight"], cfg.norm_eps)
-            stored = False
-            if decode1 and cache is not None and not cfg.qk_norm:
+            stored = kv8
+            if decode1 and cache is not None and not cfg.qk_norm and not kv8:
                 # RoPE(q) + RoPE(k)->cache + v->cache in ONE launch
                 stored = fast_rope_qkv_store(
                     q, k, v, cache.data[li, 0, 0], cache.data[li, 1, 0],
@@ -571,14 +612,13 @@ class LlamaModel:
                                    start_pos)
                     k = apply_rope(k, self.rope_cos, self.rope_sin,
                                    start_pos)
-            if cache is not None:
+            if cache is not None and not kv8:
                 if not stored:
                     cache.data[li, 0, :, start_pos:start_pos + T] = k
                     cache.data[li, 1, :, start_pos:start_pos + T] = v
                 k = cache.data[li, 0, :, : start_pos + T]
                 v = cache.data[li, 1, :, : start_pos + T]
-            att = None
-            if decode1 and cache is not None:
+            if decode1 and cache is not None and not kv8:
                 # fused GQA decode attention over the raw cache (no
                 # repeat_interleave copies, one launch)
                 att = fast_attn_decode(q, cache.data[li, 0, 0],
@@ -641,7 +681,7 @@ class LlamaModel:
 
     @torch.no_grad()
     def generate(self, prompt: torch.Tensor, max_new_tokens: int = 16,
-                 cache: Optional[KVCache] = None,
+                 cache: "KVCache | KV8Cache | None" = None,
                  eos_id: Optional[int] = None,
                  temperature: float = 0.0,
                  top_p: float = 1.0) -> torch.Tensor:
@@ -652,9 +692,8 @@ class LlamaModel:
         B, T = prompt.shape
         own_cache = cache is None
         if own_cache:
-            cache = KVCache(self.cfg, B, self.device, self.tp_size,
-                            max_seq=min(self.cfg.max_seq_len,
-                                        T + max_new_tokens))
+            cache = self.new_cache(B, max_seq=min(self.cfg.max_seq_len,
+                                                  T + max_new_tokens))
         logits = self.forward(prompt, cache, 0)
         out = prompt
         pos = T

@@ -25,7 +25,8 @@ from typing import Dict, Optional
 import torch
 import torch.distributed as dist
 
-from fma_amd.models.llama import KVCache, LlamaConfig, LlamaModel
+from fma_amd.models.llama import (LlamaConfig, LlamaModel,
+                                  check_kv_cache_dtype)
 from fma_amd.ops import actuation
 
 
@@ -38,7 +39,8 @@ class ActuationEngine:
                  use_vmm=None, chunk_bytes: int = 0, seed: int = 0,
                  init_weights: bool = True, nstreams: int = 1,
                  slab_bytes: int = None, actuation_mode: str = "arena",
-                 pack_xfer_mode=None):
+                 pack_xfer_mode=None, kv_cache_dtype: str = "auto"):
+        self.kv_cache_dtype = check_kv_cache_dtype(cfg, kv_cache_dtype)
         self.cfg = cfg
         self.device_index = device_index
         self.tp_rank = tp_rank
@@ -81,7 +83,8 @@ class ActuationEngine:
         self.timing["arena_s"] = time.perf_counter() - t0
         t1 = time.perf_counter()
         self.model = LlamaModel(cfg, self.params, self.device,
-                                tp_rank, tp_size, tp_group)
+                                tp_rank, tp_size, tp_group,
+                                kv_cache_dtype=kv_cache_dtype)
         if init_weights:
             self.model.init_weights(seed)
         if self.on_gpu:
@@ -270,7 +273,7 @@ class ActuationEngine:
                 or not self.on_gpu):
             return None
         from fma_amd.models.decode_graph import StaticDecoder as _SD
-        if mode != "1" and not _SD.supported(self.cfg):
+        if mode != "1" and not _SD.supported(self.cfg, self.kv_cache_dtype):
             # measured ROCm 7.2 graph-replay fault at large vocab
             # (decode_graph.GRAPH_SAFE_VOCAB); eager decode is clean
             return None
@@ -308,8 +311,10 @@ class ActuationEngine:
         return bytes(int(t) % 256 for t in out.tolist()).decode(
             "utf-8", errors="replace")
 
-    def new_kv_cache(self, batch: int, max_seq: Optional[int] = None) -> KVCache:
-        return KVCache(self.cfg, batch, self.device, self.tp_size, max_seq)
+    def new_kv_cache(self, batch: int, max_seq: Optional[int] = None):
+        """A cache for ``model.forward``: 16-bit, or of the engine's
+        ``kv_cache_dtype`` ("fp8" / "int8")."""
+        return self.model.new_cache(batch, max_seq)
 
     def stats(self) -> Dict[str, object]:
         return {
@@ -320,6 +325,7 @@ class ActuationEngine:
             "tp_size": self.tp_size,
             "uses_vmm": getattr(self.arena, "uses_vmm", False),
             "actuation_mode": self.actuation_mode,
+            "kv_cache_dtype": self.kv_cache_dtype,
             "graph_decode": self._decoder is not None,
             "sleep_count": self.sleep_count,
             "wake_count": self.wake_count,

@@ -17,8 +17,8 @@ endpoint for smoke traffic:
 CLI options mirror the reference's ModelServerConfig.Options surface
 (reference api/fma/v1alpha1/inferenceserverconfig_types.go:35-62):
 ``--model``, ``--port``, ``--tensor-parallel-size``, ``--enable-sleep-mode``
-(always on here), ``--max-model-len``, ``--seed``; unknown options are
-tolerated so reference ISC manifests keep working.
+(always on here), ``--max-model-len``, ``--seed``, ``--kv-cache-dtype``;
+unknown options are tolerated so reference ISC manifests keep working.
 
 TP instances: this process is rank 0; it forks ranks 1..N-1 before binding
 the port (see fma_amd/parallel/tp.py).
@@ -55,7 +55,16 @@ def parse_options(options: str) -> argparse.Namespace:
     ap.add_argument("--served-model-name", default=None)
     ap.add_argument("--start-asleep", action="store_true",
                     help="immediately sleep after load (pre-warmed instance)")
+    ap.add_argument("--kv-cache-dtype", default="auto",
+                    help="auto (the model's type), fp8 / fp8_e4m3 or int8: "
+                         "hold keys and values in 8 bits")
     args, unknown = ap.parse_known_args(options.split())
+    kv = {"fp8_e4m3": "fp8"}.get(args.kv_cache_dtype, args.kv_cache_dtype)
+    if kv not in ("auto", "fp8", "int8"):
+        print(f"[serve] --kv-cache-dtype {kv}: not served, using auto",
+              flush=True)
+        kv = "auto"
+    args.kv_cache_dtype = kv
     args.unknown = unknown
     if args.host is None:
         # node agent / launcher export the Pod's loopback identity
@@ -71,7 +80,8 @@ def _free_port() -> int:
 
 def _worker_entry(rank: int, world: int, master_port: int,
                   model_name: str, max_model_len: Optional[int],
-                  seed: int, expert_parallel: bool = False) -> None:
+                  seed: int, expert_parallel: bool = False,
+                  kv_cache_dtype: str = "auto") -> None:
     # ranks 1..N-1: build the engine shard and serve TP commands forever
     # (workers stay in the instance's process group so the launcher's
     # killpg on force-stop reaps them too)
@@ -92,7 +102,8 @@ def _worker_entry(rank: int, world: int, master_port: int,
     eng = ActuationEngine(cfg, device_index=ctx.device_index,
                           tp_rank=rank, tp_size=world,
                           tp_group=ctx.device_group, seed=seed,
-                          init_weights=checkpoint is None)
+                          init_weights=checkpoint is None,
+                          kv_cache_dtype=kv_cache_dtype)
     if checkpoint:
         eng.load_checkpoint(checkpoint)
     tp.run_worker_loop(ctx, eng)
@@ -147,7 +158,8 @@ class ServingRuntime:
             p = mp.Process(target=_worker_entry,
                            args=(r, world, master_port, args.model,
                                  args.max_model_len, args.seed,
-                                 getattr(args, "expert_parallel", False)),
+                                 getattr(args, "expert_parallel", False),
+                                 getattr(args, "kv_cache_dtype", "auto")),
                            daemon=True)
             p.start()
             self.workers.append(p)
@@ -169,7 +181,9 @@ class ServingRuntime:
         engine = ActuationEngine(cfg, device_index=ctx.device_index,
                                  tp_rank=0, tp_size=world,
                                  tp_group=ctx.device_group, seed=args.seed,
-                                 init_weights=checkpoint is None)
+                                 init_weights=checkpoint is None,
+                                 kv_cache_dtype=getattr(
+                                     args, "kv_cache_dtype", "auto"))
         if checkpoint is not None:
             t_load = engine.load_checkpoint(checkpoint)
             print(f"[serve] checkpoint {checkpoint} loaded in {t_load:.2f}s",

@@ -530,3 +530,45 @@ def test_cache_beyond_32_bit_offsets(ops):
     vh = torch.cat((torch.zeros(lo, H, hd).double(), oracle.held(v[b], "fp8")))
     want, bound = oracle.attention(q[b], kh, vh, lo + n - 1, hd ** -0.5)
     oracle.check(out[b], want, bound, BF)
+
+
+# -- the framework's own paths over it -------------------------------------------
+
+@pytest.mark.parametrize("kv", ["fp8", "int8"])
+@pytest.mark.parametrize("qk_norm", [False, True])
+def test_engine_over_an_8bit_cache(kv, qk_norm):
+    """Prompt, graph replays and a sleep/wake cycle; the replayed steps give
+    what the same steps give eagerly."""
+    from fma_amd.models.decode_graph import StaticDecoder
+    from fma_amd.models.llama import LlamaConfig
+    from fma_amd.runtime.engine import ActuationEngine
+    cfg = LlamaConfig(name="kv8", vocab_size=512, hidden_size=512,
+                      intermediate_size=768, num_layers=2, num_heads=4,
+                      num_kv_heads=2, max_seq_len=256, qk_norm=qk_norm)
+    eng = ActuationEngine(cfg, 0, seed=0, kv_cache_dtype=kv)
+    toks = torch.randint(0, 512, (1, 45), device="cuda:0",
+                         generator=torch.Generator("cuda:0").manual_seed(1))
+    out = eng.generate(toks, max_new_tokens=60)
+    assert eng.stats()["graph_decode"]
+    dec = StaticDecoder(eng.model, 1, cfg.max_seq_len)
+    assert torch.equal(dec.generate(toks, 60), out)          # eager steps
+    eng.sleep()
+    eng.wake_up()
+    assert torch.equal(eng.generate(toks, max_new_tokens=60), out)
+    # logits beside those over a 16-bit cache
+    ref = ActuationEngine(cfg, 0, seed=0)
+    a = eng.model.forward(toks, eng.new_kv_cache(1, 64), 0)
+    b = ref.model.forward(toks, ref.new_kv_cache(1, 64), 0)
+    assert (a - b).norm() < 0.1 * b.norm()
+
+
+def test_tables_of_a_model_longer_than_its_cache():
+    from fma_amd.models.llama import LlamaConfig
+    from fma_amd.runtime.engine import ActuationEngine
+    eng = ActuationEngine(LlamaConfig.tiny_qwen3(), 0, seed=0,
+                          kv_cache_dtype="fp8")
+    toks = torch.randint(0, 512, (3, 20), device="cuda:0")
+    out = eng.model.generate(toks, 30)                        # heads of 16
+    assert out.shape == (3, 50)
+    with pytest.raises(ValueError, match="tables"):
+        eng.model.forward(toks, eng.new_kv_cache(3, 300), 0)

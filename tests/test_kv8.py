@@ -253,3 +253,76 @@ def test_refusals_of_norm_rope():
     with pytest.raises(ValueError, match="tables"):
         qk_norm_rope_kv8(c, 0, torch.zeros(1, 2, 2, 8).bfloat16(), kk, v,
                          cos, sin, 0)
+
+
+# -- the framework's own paths over it -------------------------------------------
+
+def _generate(cfg, kv, prompt, n=8, batch=1):
+    from fma_amd.runtime.engine import ActuationEngine
+    eng = ActuationEngine(cfg, seed=0, kv_cache_dtype=kv)
+    return eng, eng.generate(prompt.repeat(batch, 1), max_new_tokens=n)
+
+
+@pytest.mark.parametrize("preset", ["tiny", "tiny_qwen3", "tiny_gemma",
+                                    "tiny_moe"])
+@pytest.mark.parametrize("kv", ["fp8", "int8"])
+def test_families_generate_over_an_8bit_cache(preset, kv):
+    """Logits stay near those over a 16-bit cache; prompts of one call and of
+    several, and single tokens, agree with each other."""
+    from fma_amd.models.llama import LlamaConfig
+    from fma_amd.runtime.engine import ActuationEngine
+    cfg = getattr(LlamaConfig, preset)()
+    a, b = (ActuationEngine(cfg, seed=0, kv_cache_dtype=x)
+            for x in ("auto", kv))
+    assert b.stats()["kv_cache_dtype"] == kv
+    toks = torch.randint(0, cfg.vocab_size, (2, 70),
+                         generator=torch.Generator().manual_seed(1))
+    ca, cb = a.new_kv_cache(2, 80), b.new_kv_cache(2, 80)
+    assert isinstance(cb, KV8Cache) and cb.fmt == kv
+    la = a.model.forward(toks, ca, 0)
+    lb = b.model.forward(toks, cb, 0)
+    # a key or value moves by at most 2^-4 of its size, two layers deep;
+    # a wrong token, position or head moves the logits by their own size
+    assert (la - lb).norm() < 0.1 * la.norm()
+    # rows over whole blocks do not depend on the split of the prompt
+    cc = b.new_kv_cache(2, 80)
+    b.model.forward(toks[:, :64], cc, 0)
+    lc = b.model.forward(toks[:, 64:], cc, 64)
+    assert (lc - lb[:, 64:]).norm() < 2e-2 * lb[:, 64:].norm()
+    out = b.generate(toks, max_new_tokens=5)
+    assert out.shape == (2, 75)
+
+
+def test_static_decoder_over_an_8bit_cache():
+    from fma_amd.models.decode_graph import StaticDecoder
+    from fma_amd.models.llama import LlamaConfig
+    for cfg in (LlamaConfig.tiny(), LlamaConfig.tiny_qwen3()):
+        eng, want = _generate(cfg, "fp8", torch.arange(1, 31)[None], 40)
+        assert StaticDecoder.supported(cfg, "fp8")
+        dec = StaticDecoder(eng.model, 1, 128)
+        for _ in range(2):
+            assert torch.equal(dec.generate(torch.arange(1, 31)[None], 40),
+                               want)
+
+
+def test_option_reaches_the_engine():
+    from fma_amd.models.llama import LlamaConfig
+    from fma_amd.runtime.engine import ActuationEngine
+    from fma_amd.runtime.server import ServingRuntime, parse_options
+    assert parse_options("--model tiny").kv_cache_dtype == "auto"
+    for given, want in (("fp8", "fp8"), ("fp8_e4m3", "fp8"),
+                        ("int8", "int8"), ("fp8_e5m2", "auto")):
+        args = parse_options(f"--model tiny --kv-cache-dtype {given}")
+        assert args.kv_cache_dtype == want
+    rt = ServingRuntime(parse_options("--model tiny --kv-cache-dtype fp8"))
+    try:
+        assert rt.rt.stats()["kv_cache_dtype"] == "fp8"
+        assert len(rt.rt.generate_text("hello", 3)) >= 0
+    finally:
+        rt.close()
+    with pytest.raises(ValueError):
+        ActuationEngine(LlamaConfig.tiny(), kv_cache_dtype="int4")
+    cfg = LlamaConfig.tiny()
+    cfg.dtype = torch.float32
+    with pytest.raises(ValueError):
+        ActuationEngine(cfg, kv_cache_dtype="fp8")
