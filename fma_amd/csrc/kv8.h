@@ -80,7 +80,7 @@ extern "C" hipError_t fma_launch_kv8_read(FmaKv8Layer c, const int* start,
                                           int length_i, int n, void* ko,
                                           void* vo, hipStream_t stream);
 
-// partials: fp32 [rows, splits, hdp + 2] where splits > 1
+// partials: fp32, rows * splits * (hdp + 2) of them where splits > 1
 extern "C" int fma_kv8_attn_splits(const FmaKv8Layer* c, int T, int q_heads,
                                    int max_len, int cus);
 extern "C" hipError_t fma_launch_kv8_attention(FmaKv8Layer c, FmaKv8Span span,

@@ -16,6 +16,7 @@ typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int BLK = FMA_KV8_BLOCK;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxSplits = 128;
 constexpr float kMinAmax = 7.888609052210118e-31f;  // 2^-100
 
 // ---------------------------------------------------------------------------
@@ -569,12 +570,12 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(
 // Reading back: one workgroup a block of one kv head, through LDS because a
 // token's values do not lie together in V.
 
-template <typename E, bool FP8>
+template <int NS, typename E, bool FP8>
 __global__ __launch_bounds__(256) void kv8_read_kernel(
     FmaKv8Layer c, const int* start, int start_i, const int* length,
     int length_i, int n, uint16_t* ko, uint16_t* vo, int blocks) {
-  extern __shared__ uint16_t tile[];  // [BLK][pitch]
-  const int pitch = c.hdp + 8;
+  constexpr int HDP = NS * 32;
+  __shared__ uint16_t tile[BLK][HDP + 8];
   const int j = blockIdx.x % blocks;
   const int bh = blockIdx.x / blocks;
   const int b = bh / c.kv_heads, h = bh - b * c.kv_heads;
@@ -583,8 +584,8 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(
   len = min(max(len, 0), c.max_seq);
   const int blk = s0 / BLK + j;
   const int lo = max(s0, blk * BLK);
-  const long long hi_l = min(static_cast<long long>(s0) + n, (blk + 1LL) * BLK);
-  const int hi = static_cast<int>(hi_l);
+  const int hi = static_cast<int>(
+      min(static_cast<long long>(s0) + n, (blk + 1LL) * BLK));
   if (hi <= lo) return;
   const int which = blockIdx.y;
   uint16_t* const out = which ? vo : ko;
@@ -594,10 +595,12 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(
                                  static_cast<long long>(bh) * c.nblk + blk];
     const unsigned char* const at =
         c.codes + which * c.codes_v +
-        (static_cast<long long>(bh) * c.nblk + blk) * BLK * c.hdp;
-    for (int u = threadIdx.x; u < c.hdp * 2; u += 256) {
+        (static_cast<long long>(bh) * c.nblk + blk) * BLK * HDP;
+#pragma unroll
+    for (int u = threadIdx.x; u < HDP * 2; u += 256) {
       const int l = u & 63, chunk = u >> 6, g = l >> 4, m = l & 15;
       const u32x4 w = *reinterpret_cast<const u32x4*>(at + u * 16);
+      uint16_t x[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const uint32_t byte = (w[e >> 2] >> (8 * (e & 3))) & 255u;
@@ -606,28 +609,59 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(
           f = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(byte), 0);
         else
           f = static_cast<float>(static_cast<int>(byte) - 128);
-        const int tok = which ? 16 * ((e >> 2) & 1) + 4 * g + (e & 3)
-                              : 16 * (e >> 3) + m;
-        const int d = which ? 32 * chunk + 16 * (e >> 3) + m
-                            : 32 * chunk + 8 * g + (e & 7);
-        tile[tok * pitch + d] = E::from_f(f * scale);
+        x[e] = E::from_f(f * scale);
+      }
+      if (which) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          tile[16 * ((e >> 2) & 1) + 4 * g + (e & 3)]
+              [32 * chunk + 16 * (e >> 3) + m] = x[e];
+      } else {
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          u16x8 v;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = x[8 * a + e];
+          *reinterpret_cast<u16x8*>(&tile[16 * a + m][32 * chunk + 8 * g]) = v;
+        }
       }
     }
   } else if (any) {
     const uint16_t* const t =
         static_cast<const uint16_t*>(c.tail) + which * c.tail_v +
-        (static_cast<long long>(bh) * 2 + (blk & 1)) * BLK * c.hdp;
-    for (int i = threadIdx.x; i < BLK * c.hdp; i += 256) {
-      const int tok = i / c.hdp, d = i - tok * c.hdp;
-      tile[tok * pitch + d] = t[which ? vidx(tok, d) : kidx(tok, d)];
+        (static_cast<long long>(bh) * 2 + (blk & 1)) * BLK * HDP;
+#pragma unroll
+    for (int u = threadIdx.x; u < HDP * 4; u += 256) {
+      // eight values that lie together: of one token, or of eight
+      const u16x8 v = *reinterpret_cast<const u16x8*>(t + u * 8);
+      const int e = u & 1, l = (u >> 1) & 63, chunk = u >> 7;
+      const int g = l >> 4, m = l & 15;
+      if (which) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          tile[16 * (i >> 2) + 4 * g + (i & 3)][32 * chunk + 16 * e + m] = v[i];
+      } else {
+        *reinterpret_cast<u16x8*>(&tile[16 * e + m][32 * chunk + 8 * g]) = v;
+      }
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < (hi - lo) * c.hd; i += 256) {
-    const int tok = i / c.hd, d = i - tok * c.hd;
-    const int p = lo + tok;
-    out[((static_cast<long long>(b) * n + (p - s0)) * c.kv_heads + h) * c.hd +
-        d] = p < len ? tile[(p - blk * BLK) * pitch + d] : 0;
+  const bool vec = c.hd % 8 == 0;
+  for (int u = threadIdx.x; u < (hi - lo) * NS * 4; u += 256) {
+    const int p = lo + u / (NS * 4), d = u % (NS * 4) * 8;
+    if (d >= c.hd) continue;
+    uint16_t* const o =
+        out + ((static_cast<long long>(b) * n + (p - s0)) * c.kv_heads + h) *
+                  c.hd + d;
+    u16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (p < len) v = *reinterpret_cast<const u16x8*>(&tile[p - blk * BLK][d]);
+    if (vec) {
+      *reinterpret_cast<u16x8*>(o) = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (d + i < c.hd) o[i] = v[i];
+    }
   }
 }
 
@@ -668,7 +702,8 @@ struct AttnArgs {
   FmaKv8Span sp;
   FmaRows q;
   void* out;
-  float* partials;
+  float* partials;  // [rows, splits, HDP]
+  float* stats;     // [rows, splits, 2]: reference and sum
   float scale;  // of the scores, times log2(e)
   int q_heads, group, rows, tiles, splits;
 };
@@ -693,6 +728,12 @@ __device__ inline f32x4 mfma16(u16x8 a, u16x8 b, f32x4 acc) {
         __builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), acc, 0, 0, 0);
 }
 
+// Maximum over the four lanes 16 g + row that hold a row.
+__device__ inline float row_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+
 // One wave's softmax and output state for 16 query rows.
 template <int NS>
 struct RowState {
@@ -710,23 +751,31 @@ struct RowState {
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[n][r] *= f;
   }
-  // Scores in units of log2; on return the weights, with the sum advanced.
-  // The reference moves only when a score passes it by 2^8, which fp16
-  // weights and fp32 sums have room for; so the output is rarely rescaled.
-  __device__ void weigh(f32x4 (&x)[2]) {
+  // x: products of a block, f: what makes them log2 scores. On return the
+  // weights, with the sum advanced. The reference moves only when a score
+  // passes it by 2^8, which fp16 weights and fp32 sums have room for: the
+  // output is rarely rescaled, and while no lane asks for it, no value has to
+  // cross lanes.
+  template <bool MASK>
+  __device__ void weigh(f32x4 (&x)[2], float f, int left) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[a][r] *= f;
+        if (MASK && 16 * a + r >= left) x[a][r] = -INFINITY;
+      }
     float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
                       fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const bool move = top > m + 8.0f || (m == -INFINITY && top > m);
-    if (__any(move)) {
-      const float next = move ? top : m;
-      const float f = move ? exp2f(m - next) : 1.0f;
+    if (__any(top > m + 8.0f)) {
+      top = row_max(top);
+      const float next = top > m + 8.0f ? top : m;
+      const float g = next == m ? 1.0f : exp2f(m - next);
       m = next;
-      l *= f;
-      times(f);
+      l *= g;
+      times(g);
     }
-    const float ref = m == -INFINITY ? 0.0f : m;
+    const float ref = MASK && m == -INFINITY ? 0.0f : m;
     float sum = 0.0f;
 #pragma unroll
     for (int a = 0; a < 2; ++a)
@@ -739,76 +788,161 @@ struct RowState {
   }
 };
 
-// Four waves share 16 rows and take the blocks of a split in turn.
+// Where a tile of query rows reads its keys: its sequence, its blocks held as
+// codes, and whether it sees the incomplete block.
+struct Reach {
+  Span s;
+  int full, lo, hi;
+  bool tail;
+};
+__device__ inline Reach reach_of(const AttnArgs& A, int b, int row0, int rows,
+                                 int split) {
+  Reach r;
+  r.s = span_of(A.sp, b, A.c.max_seq);
+  const int t_first = row0 / A.group;
+  const int t_last =
+      min((min(row0 + rows, A.rows) - 1) / A.group, r.s.count - 1);
+  const int most = t_first < r.s.count ? r.s.start + t_last + 1 : 0;
+  r.full = r.s.end / BLK;
+  const long long nb = min(r.full, (most + BLK - 1) / BLK);
+  r.lo = static_cast<int>(nb * split / A.splits);
+  r.hi = static_cast<int>(nb * (split + 1) / A.splits);
+  r.tail = most > r.full * BLK && split == A.splits - 1;
+  return r;
+}
+
+// A query row's values 32 ks + 8 g ..: as they are, and as fp16.
+template <int NS, typename E>
+__device__ inline void load_query(const AttnArgs& A, const uint16_t* row,
+                                  bool live, int g, u16x8 (&raw)[NS]) {
+#pragma unroll
+  for (int ks = 0; ks < NS; ++ks) {
+    const int d = 32 * ks + 8 * g;
+    raw[ks] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    if (live && d < A.c.hd) {
+      if (A.q.vec) {
+        raw[ks] = *reinterpret_cast<const u16x8*>(row + d);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (d + i < A.c.hd) raw[ks][i] = row[d + i];
+      }
+    }
+  }
+}
+// Returns what makes products of codes log2 scores, but for K's scale.
+template <int NS, typename E>
+__device__ inline float query_fp16(const AttnArgs& A, const u16x8 (&raw)[NS],
+                                   h8 (&q)[NS]) {
+  float top = 0.0f;
+#pragma unroll
+  for (int ks = 0; ks < NS; ++ks)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(E::to_f(raw[ks][i])));
+  top = row_max(top);
+  // 2^-e brings the row's largest into [2^9, 2^10)
+  int e = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 9;
+  e = top == 0.0f ? 0 : min(max(e, -100), 100);
+  const float mul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+  for (int ks = 0; ks < NS; ++ks)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      q[ks][i] = static_cast<_Float16>(E::to_f(raw[ks][i]) * mul);
+  return A.scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+
+// The running reference of V's scales. It moves where fp16 has no room for
+// the ratio to it; down only as far as fp32 sums cannot overflow.
+struct ScaleRef {
+  float ref, most;
+  // true: multiply the outputs by *f
+  __device__ bool move(float scale, float* f) {
+    if (scale <= ref * 64.0f &&
+        !(scale < ref * 0.015625f && scale >= most * 5.4e-20f))
+      return false;
+    *f = ref != 0.0f ? ref / scale : 1.0f;
+    ref = scale;
+    most = fmaxf(most, scale);
+    return true;
+  }
+};
+
+// The incomplete block, raw, for 16 rows. Its weights go in as two 16-bit
+// parts: a single bf16 would cost as much as the result's rounding.
+template <int NS, typename E>
+__device__ inline void tail_step(const AttnArgs& A, const Reach& R, int bh,
+                                 int lane, const u16x8 (&q)[NS], int seen,
+                                 RowState<NS>& st) {
+  const int g = lane >> 4;
+  const uint16_t* const kt =
+      static_cast<const uint16_t*>(A.c.tail) +
+      (static_cast<long long>(bh) * 2 + (R.full & 1)) * BLK * NS * 32 +
+      lane * 16;
+  const uint16_t* const vt = kt + A.c.tail_v;
+  f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+  for (int ks = 0; ks < NS; ++ks)
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+      x[a] = mfma16<E>(*reinterpret_cast<const u16x8*>(kt + ks * 1024 + a * 8),
+                       q[ks], x[a]);
+  st.template weigh<true>(x, A.scale, seen - R.full * BLK - 4 * g);
+  u16x8 hi, lo;
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint16_t u = E::from_f(x[a][r]);
+      hi[4 * a + r] = u;
+      lo[4 * a + r] = E::from_f(x[a][r] - E::to_f(u));
+    }
+  const int held = R.s.end - R.full * BLK - 4 * g;
+#pragma unroll
+  for (int n = 0; n < 2 * NS; ++n) {
+    u16x8 v = *reinterpret_cast<const u16x8*>(vt + (n >> 1) * 1024 +
+                                              (n & 1) * 8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = 16 * (i >> 2) + (i & 3) < held ? tame<E>(v[i]) : 0;
+    st.o[n] = mfma16<E>(v, hi, st.o[n]);
+    st.o[n] = mfma16<E>(v, lo, st.o[n]);
+  }
+}
+
+// Few rows: four waves share 16 rows and take the blocks of a split in turn,
+// each straight from memory into the matrix unit's operands, the next block
+// on its way meanwhile.
 template <int NS, bool FP8, typename E>
-__global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs A) {
+__global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(AttnArgs A) {
   constexpr int HDP = NS * 32;
   __shared__ float s_o[4][16][HDP + 4];
   __shared__ float s_m[4][16], s_l[4][16];
   const FmaKv8Layer& c = A.c;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g = lane >> 4, n16 = lane & 15;
-  const int split = blockIdx.x % A.splits;
-  const int rest = blockIdx.x / A.splits;
-  const int tile = rest % A.tiles;
-  const int bh = rest / A.tiles;
+  const int heads = c.batch * c.kv_heads;
+  const int bh = blockIdx.x % heads;
+  const int rest = blockIdx.x / heads;
+  const int split = rest % A.splits, tile = rest / A.splits;
   const int b = bh / c.kv_heads, h = bh - b * c.kv_heads;
-  const Span s = span_of(A.sp, b, c.max_seq);
+  const Reach R = reach_of(A, b, tile * 16, 16, split);
 
   const int row = tile * 16 + n16;
   const int t = row / A.group, hq = h * A.group + (row - t * A.group);
-  const bool live = row < A.rows && t < s.count;
-  const int seen = live ? s.start + t + 1 : 0;       // keys of this row
-  const int t_last = min(min(tile * 16 + 15, A.rows - 1) / A.group,
-                         s.count - 1);
-  const int t_first = tile * 16 / A.group;
-  const int most = t_first < s.count ? s.start + t_last + 1 : 0;
-  const int full = s.end / BLK;                      // blocks held as codes
-  const int nb = min(full, (most + BLK - 1) / BLK);
-  const int blk_lo = static_cast<int>(static_cast<long long>(nb) * split / A.splits);
-  const int blk_hi = static_cast<int>(static_cast<long long>(nb) * (split + 1) / A.splits);
-  const bool has_tail = most > full * BLK && split == A.splits - 1;
+  const bool live = row < A.rows && t < R.s.count;
+  const int seen = live ? R.s.start + t + 1 : 0;  // keys of this row
 
   RowState<NS> st;
   st.clear();
 
-  if (blk_lo < blk_hi || has_tail) {
-    // this row's query, as it is and as fp16
+  if (R.lo < R.hi || R.tail) {
     const uint16_t* const qrow = static_cast<const uint16_t*>(A.q.p) +
                                  b * A.q.sb + t * A.q.st + hq * A.q.sh;
     u16x8 qraw[NS];
-    float top = 0.0f;
-#pragma unroll
-    for (int ks = 0; ks < NS; ++ks) {
-      const int d = 32 * ks + 8 * g;
-      qraw[ks] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
-      if (live && d < c.hd) {
-        if (A.q.vec) {
-          qraw[ks] = *reinterpret_cast<const u16x8*>(qrow + d);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (d + i < c.hd) qraw[ks][i] = qrow[d + i];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        top = fmaxf(top, fabsf(E::to_f(qraw[ks][i])));
-    }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    // 2^-e brings the row's largest into [2^9, 2^10)
-    int e = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 9;
-    e = top == 0.0f ? 0 : min(max(e, -100), 100);
-    const float qmul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-    const float qscale =
-        A.scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-    h8 qf[NS];
-#pragma unroll
-    for (int ks = 0; ks < NS; ++ks)
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        qf[ks][i] = static_cast<_Float16>(E::to_f(qraw[ks][i]) * qmul);
+    h8 q[NS];
+    load_query<NS, E>(A, qrow, live, g, qraw);
+    const float qscale = query_fp16<NS, E>(A, qraw, q);
 
     const unsigned char* const kc =
         c.codes + static_cast<long long>(bh) * c.nblk * BLK * HDP + lane * 16;
@@ -816,7 +950,7 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs A) {
     const float* const ksc = c.scales + static_cast<long long>(bh) * c.nblk;
     const float* const vsc = ksc + c.scales_v;
 
-    float vref = 0.0f, vmost = 0.0f;
+    ScaleRef vs{0.0f, 0.0f};
     u32x4 kr[NS], vr[NS];
     auto load = [&](int blk) {
       const long long at = static_cast<long long>(blk) * BLK * HDP;
@@ -827,39 +961,26 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs A) {
       for (int i = 0; i < NS; ++i)
         vr[i] = *reinterpret_cast<const u32x4*>(vc + at + i * 1024);
     };
-    int blk = blk_lo + wave;
-    if (blk < blk_hi) load(blk);
-    for (; blk < blk_hi; blk += 4) {
+    int blk = R.lo + wave;
+    if (blk < R.hi) load(blk);
+    for (; blk < R.hi; blk += 4) {
       const float kscale = ksc[blk], vscale = vsc[blk];
       f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
       for (int ks = 0; ks < NS; ++ks) {
         x[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-            decode8(kr[ks][0], kr[ks][1], 1.0f, FP8), qf[ks], x[0], 0, 0, 0);
+            decode8(kr[ks][0], kr[ks][1], 1.0f, FP8), q[ks], x[0], 0, 0, 0);
         x[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-            decode8(kr[ks][2], kr[ks][3], 1.0f, FP8), qf[ks], x[1], 0, 0, 0);
+            decode8(kr[ks][2], kr[ks][3], 1.0f, FP8), q[ks], x[1], 0, 0, 0);
       }
       u32x4 v_now[NS];
 #pragma unroll
       for (int i = 0; i < NS; ++i) v_now[i] = vr[i];
-      if (blk + 4 < blk_hi) load(blk + 4);
-      const float f = kscale * qscale;
-      const int left = seen - blk * BLK - 4 * g;  // tokens of this lane's on
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          x[a][r] = 16 * a + r < left ? x[a][r] * f : -INFINITY;
-      st.weigh(x);
-      // move the reference of V's scales where fp16 has no room for the
-      // ratio; down only as far as fp32 sums cannot overflow
-      if (!(vscale <= vref * 64.0f) ||
-          (vscale < vref * 0.015625f && vscale >= vmost * 5.4e-20f)) {
-        if (vref != 0.0f) st.times(vref / vscale);
-        vref = vscale;
-        vmost = fmaxf(vmost, vscale);
-      }
-      const float ratio = vscale / vref;
+      if (blk + 4 < R.hi) load(blk + 4);
+      st.template weigh<true>(x, kscale * qscale, seen - blk * BLK - 4 * g);
+      float f;
+      if (vs.move(vscale, &f)) st.times(f);
+      const float ratio = vscale / vs.ref;
       h8 p;
 #pragma unroll
       for (int a = 0; a < 2; ++a)
@@ -877,51 +998,8 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs A) {
             0, 0, 0);
       }
     }
-    st.times(vref);
-
-    if (has_tail && wave == 3) {
-      // the block that is not complete, raw. Its weights go in as two 16-bit
-      // parts: a single bf16 would cost as much as the result's rounding.
-      const uint16_t* const kt =
-          static_cast<const uint16_t*>(c.tail) +
-          (static_cast<long long>(bh) * 2 + (full & 1)) * BLK * HDP + lane * 16;
-      const uint16_t* const vt = kt + c.tail_v;
-      f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-#pragma unroll
-      for (int ks = 0; ks < NS; ++ks)
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-          x[a] = mfma16<E>(
-              *reinterpret_cast<const u16x8*>(kt + ks * 1024 + a * 8),
-              qraw[ks], x[a]);
-      const int left = seen - full * BLK - 4 * g;
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          x[a][r] = 16 * a + r < left ? x[a][r] * A.scale : -INFINITY;
-      st.weigh(x);
-      u16x8 hi, lo;
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint16_t u = E::from_f(x[a][r]);
-          hi[4 * a + r] = u;
-          lo[4 * a + r] = E::from_f(x[a][r] - E::to_f(u));
-        }
-      const int held = s.end - full * BLK - 4 * g;
-#pragma unroll
-      for (int n = 0; n < 2 * NS; ++n) {
-        u16x8 vv = *reinterpret_cast<const u16x8*>(vt + (n >> 1) * 1024 +
-                                                   (n & 1) * 8);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          vv[i] = 16 * (i >> 2) + (i & 3) < held ? tame<E>(vv[i]) : 0;
-        st.o[n] = mfma16<E>(vv, hi, st.o[n]);
-        st.o[n] = mfma16<E>(vv, lo, st.o[n]);
-      }
-    }
+    st.times(vs.ref);
+    if (R.tail && wave == 3) tail_step<NS, E>(A, R, bh, lane, qraw, seen, st);
   }
 
   // join the four waves
@@ -958,33 +1036,270 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs A) {
         static_cast<uint16_t*>(A.out)[at * c.hd + d] =
             E::from_f(sum == 0.0f ? 0.0f : o / sum);
     } else {
-      float* const part = A.partials + (at * A.splits + split) * (HDP + 2);
-      part[d] = o;
+      A.partials[(at * A.splits + split) * HDP + d] = o;
       if (d == 0) {
-        part[HDP] = m;
-        part[HDP + 1] = sum;
+        float* const st = A.stats + (at * A.splits + split) * 2;
+        st[0] = m;
+        st[1] = sum;
       }
     }
   }
 }
 
-// Joins the splits of a row, always in the same order.
-template <typename E>
-__global__ __launch_bounds__(256) void kv8_join_kernel(
-    const float* partials, uint16_t* out, long long rows, int splits, int hd,
-    int hdp) {
-  const long long row = blockIdx.x;
-  const float* const p = partials + row * splits * (hdp + 2);
-  float m = -INFINITY;
-  for (int s = 0; s < splits; ++s) m = fmaxf(m, p[s * (hdp + 2) + hdp]);
-  const float ref = m == -INFINITY ? 0.0f : m;
-  for (int d = threadIdx.x; d < hd; d += blockDim.x) {
-    float o = 0.0f, sum = 0.0f;
-    for (int s = 0; s < splits; ++s) {
-      const float f = exp2f(p[s * (hdp + 2) + hdp] - ref);
-      o += p[s * (hdp + 2) + d] * f;
-      sum += p[s * (hdp + 2) + hdp + 1] * f;
+// Many rows: each of four waves has 16 * NR rows of its own, and all take the
+// same blocks, which go through LDS (two of them, one being filled).
+template <int NS, bool FP8, typename E, int NR>
+__global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
+  constexpr int HDP = NS * 32;
+  constexpr int UNITS = 2 * NS * 64;  // of 16 bytes in a block of K and V
+  __shared__ u32x4 s_kv[2][UNITS];
+  const FmaKv8Layer& c = A.c;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g = lane >> 4, n16 = lane & 15;
+  const int heads = c.batch * c.kv_heads;
+  const int bh = blockIdx.x % heads;
+  const int rest = blockIdx.x / heads;
+  // the tiles that see most first
+  const int split = rest / A.tiles, tile = A.tiles - 1 - rest % A.tiles;
+  const int b = bh / c.kv_heads, h = bh - b * c.kv_heads;
+  constexpr int ROWS = 64 * NR;
+  const Reach R = reach_of(A, b, tile * ROWS, ROWS, split);
+
+  RowState<NS> st[NR];
+  int seen[NR];
+  const uint16_t* qrow[NR];
+  bool live[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    st[r].clear();
+    const int row = tile * ROWS + (wave * NR + r) * 16 + n16;
+    const int t = row / A.group, hq = h * A.group + (row - t * A.group);
+    live[r] = row < A.rows && t < R.s.count;
+    seen[r] = live[r] ? R.s.start + t + 1 : 0;
+    qrow[r] = static_cast<const uint16_t*>(A.q.p) + b * A.q.sb + t * A.q.st +
+              hq * A.q.sh;
+  }
+  // blocks that every row of the wave sees whole
+  const int first = (tile * ROWS + wave * NR * 16) / A.group;
+  const int last_row = min(tile * ROWS + (wave + 1) * NR * 16, A.rows) - 1;
+  const bool whole_wave =
+      tile * ROWS + (wave + 1) * NR * 16 <= A.rows &&
+      last_row / A.group < R.s.count;
+  const int clear = whole_wave ? (R.s.start + first + 1) / BLK : 0;
+
+  if (R.lo < R.hi) {
+    h8 q[NR][NS];
+    float qscale[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      u16x8 raw[NS];
+      load_query<NS, E>(A, qrow[r], live[r], g, raw);
+      qscale[r] = query_fp16<NS, E>(A, raw, q[r]);
     }
+    const unsigned char* const kc =
+        c.codes + static_cast<long long>(bh) * c.nblk * BLK * HDP;
+    const float* const ksc = c.scales + static_cast<long long>(bh) * c.nblk;
+    const float* const vsc = ksc + c.scales_v;
+    constexpr int EACH = (UNITS + 255) / 256;
+    u32x4 next[EACH];
+    auto load = [&](int blk) {
+      const unsigned char* const at = kc + static_cast<long long>(blk) * BLK * HDP;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int u = threadIdx.x + i * 256;
+        if (UNITS % 256 == 0 || u < UNITS)
+          next[i] = *reinterpret_cast<const u32x4*>(
+              at + (u < UNITS / 2 ? 0 : c.codes_v - BLK * HDP) +
+              static_cast<long long>(u) * 16);
+      }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int u = threadIdx.x + i * 256;
+        if (UNITS % 256 == 0 || u < UNITS) s_kv[buf][u] = next[i];
+      }
+    };
+    load(R.lo);
+    store(0);
+    __syncthreads();
+    ScaleRef vs{0.0f, 0.0f};
+    for (int blk = R.lo; blk < R.hi; ++blk) {
+      const int buf = (blk - R.lo) & 1;
+      if (blk + 1 < R.hi) load(blk + 1);
+      const float kscale = ksc[blk], vscale = vsc[blk];
+      f32x4 x[NR][2];
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+        x[r][0] = x[r][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int ks = 0; ks < NS; ++ks) {
+        const u32x4 w = s_kv[buf][ks * 64 + lane];
+        const h8 k0 = decode8(w[0], w[1], 1.0f, FP8);
+        const h8 k1 = decode8(w[2], w[3], 1.0f, FP8);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          x[r][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[r][ks],
+                                                           x[r][0], 0, 0, 0);
+          x[r][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[r][ks],
+                                                           x[r][1], 0, 0, 0);
+        }
+      }
+      if (blk < clear) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+          st[r].template weigh<false>(x[r], kscale * qscale[r], 0);
+      } else {
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+          st[r].template weigh<true>(x[r], kscale * qscale[r],
+                                     seen[r] - blk * BLK - 4 * g);
+      }
+      float f;
+      if (vs.move(vscale, &f)) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) st[r].times(f);
+      }
+      const float ratio = vscale / vs.ref;
+      h8 p[NR];
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            p[r][4 * a + i] =
+                static_cast<_Float16>(FP8 ? x[r][a][i] : x[r][a][i] * ratio);
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const u32x4 w = s_kv[buf][(NS + i) * 64 + lane];
+        const h8 v0 = decode8(w[0], w[1], ratio, FP8);
+        const h8 v1 = decode8(w[2], w[3], ratio, FP8);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          st[r].o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              v0, p[r], st[r].o[2 * i], 0, 0, 0);
+          st[r].o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              v1, p[r], st[r].o[2 * i + 1], 0, 0, 0);
+        }
+      }
+      if (blk + 1 < R.hi) store(buf ^ 1);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) st[r].times(vs.ref);
+  }
+  if (R.tail) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      u16x8 raw[NS];
+      load_query<NS, E>(A, qrow[r], live[r], g, raw);
+      tail_step<NS, E>(A, R, bh, lane, raw, seen[r], st[r]);
+    }
+  }
+
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const int row = tile * ROWS + (wave * NR + r) * 16 + n16;
+    if (row >= A.rows) continue;
+    float l = st[r].l;
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    const int t = row / A.group, hq = h * A.group + (row - t * A.group);
+    const long long at =
+        (static_cast<long long>(b) * A.sp.T + t) * A.q_heads + hq;
+    if (A.splits == 1) {
+      uint16_t* const out = static_cast<uint16_t*>(A.out) + at * c.hd;
+#pragma unroll
+      for (int n = 0; n < 2 * NS; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = 16 * n + 4 * g + i;
+          if (d < c.hd)
+            out[d] = E::from_f(l == 0.0f ? 0.0f : st[r].o[n][i] / l);
+        }
+    } else {
+      float* const part = A.partials + (at * A.splits + split) * HDP;
+#pragma unroll
+      for (int n = 0; n < 2 * NS; ++n)
+        *reinterpret_cast<f32x4*>(part + 16 * n + 4 * g) = st[r].o[n];
+      if (g == 0) {
+        float* const s2 = A.stats + (at * A.splits + split) * 2;
+        s2[0] = st[r].m;
+        s2[1] = l;
+      }
+    }
+  }
+}
+
+// Joins the splits of a row, always in the same order: one workgroup a row,
+// as many splits at once as have a lane for each four values. The values are
+// asked for before the weights are known.
+template <int NS, typename E>
+__global__ __launch_bounds__(256) void kv8_join_kernel(const float* partials,
+                                                       const float* stats,
+                                                       uint16_t* out,
+                                                       int splits, int hd) {
+  constexpr int HDP = NS * 32, LANES = HDP / 4, GROUPS = 256 / LANES;
+  constexpr int TURNS = (kMaxSplits + GROUPS - 1) / GROUPS;
+  __shared__ float s_w[kMaxSplits];
+  __shared__ f32x4 s_o[GROUPS][LANES];
+  __shared__ float s_sum;
+  const long long row = blockIdx.x;
+  const int tid = threadIdx.x, grp = tid / LANES, lane = tid % LANES;
+  const float* const p = partials + row * splits * HDP + lane * 4;
+  f32x4 x[TURNS];
+#pragma unroll
+  for (int i = 0; i < TURNS; ++i) {
+    const int s = grp + i * GROUPS;
+    x[i] = f32x4{0, 0, 0, 0};
+    if (grp < GROUPS && s < splits)
+      x[i] = *reinterpret_cast<const f32x4*>(p + static_cast<long long>(s) * HDP);
+  }
+  if (tid < 64) {
+    float m[2], l[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int s = tid + 64 * i;
+      const float* const st = stats + (row * splits + s) * 2;
+      m[i] = s < splits ? st[0] : -INFINITY;
+      l[i] = s < splits ? st[1] : 0.0f;
+    }
+    float top = fmaxf(m[0], m[1]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float w = exp2f(m[i] - ref);
+      s_w[tid + 64 * i] = w;
+      sum += w * l[i];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if (tid == 0) s_sum = sum;
+  }
+  __syncthreads();
+  if (grp < GROUPS) {
+    f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+      const int s = grp + i * GROUPS;
+      if (s < splits) {
+        const float w = s_w[s];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = fmaf(x[i][r], w, o[r]);
+      }
+    }
+    s_o[grp][lane] = o;
+  }
+  __syncthreads();
+  for (int d = tid; d < hd; d += 256) {
+    float o = 0.0f;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) o += s_o[i][d >> 2][d & 3];
+    const float sum = s_sum;
     out[row * hd + d] = E::from_f(sum == 0.0f ? 0.0f : o / sum);
   }
 }
@@ -1081,23 +1396,34 @@ extern "C" hipError_t fma_launch_kv8_read(FmaKv8Layer c, const int* start,
   const long long groups = static_cast<long long>(c.batch) * c.kv_heads * blocks;
   if (groups > 0x7fffffffLL) return hipErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(groups), 2);
-  const size_t lds = static_cast<size_t>(BLK) * (c.hdp + 8) * 2;
-  FMA_BY_TYPE16(c.bf16, FMA_BY_BOOL(c.fp8, FP8,
-      return launch(kv8_read_kernel<E, FP8>, grid, 256, lds, stream, c, start,
-                    start_i, length, length_i, n, static_cast<uint16_t*>(ko),
-                    static_cast<uint16_t*>(vo), blocks)));
+  FMA_BY_TYPE16(c.bf16, FMA_BY_BOOL(c.fp8, FP8, FMA_BY_WIDTH(c.hdp,
+      return launch(kv8_read_kernel<NS, E, FP8>, grid, 256, 0, stream, c,
+                    start, start_i, length, length_i, n,
+                    static_cast<uint16_t*>(ko), static_cast<uint16_t*>(vo),
+                    blocks))));
 }
+
+namespace {
+// Rows of one kv head that a workgroup takes: 16 while they are few, then 64
+// times NR.
+constexpr int kFewRows = 32;
+constexpr int many_nr(int ns) { return ns <= 4 ? 2 : 1; }
+int tile_rows(long long rows, int hdp) {
+  return rows <= kFewRows ? 16 : 64 * many_nr(hdp / 32);
+}
+}  // namespace
 
 extern "C" int fma_kv8_attn_splits(const FmaKv8Layer* c, int T, int q_heads,
                                    int max_len, int cus) {
   const long long rows = static_cast<long long>(T) * (q_heads / c->kv_heads);
+  const int tile = tile_rows(rows, c->hdp);
   const long long groups =
-      (rows + 15) / 16 * c->batch * c->kv_heads;
+      (rows + tile - 1) / tile * c->batch * c->kv_heads;
   const int nb = max_len / BLK;
   // two workgroups a CU, and at least a block for each wave
   long long splits = groups > 0 ? 2LL * cus / groups : 1;
   if (splits > nb / 4) splits = nb / 4;
-  return splits < 1 ? 1 : splits > 64 ? 64 : static_cast<int>(splits);
+  return splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : static_cast<int>(splits);
 }
 
 extern "C" hipError_t fma_launch_kv8_attention(FmaKv8Layer c, FmaKv8Span span,
@@ -1112,26 +1438,34 @@ extern "C" hipError_t fma_launch_kv8_attention(FmaKv8Layer c, FmaKv8Span span,
   a.q = q;
   a.out = out;
   a.partials = partials;
+  a.stats = partials + static_cast<long long>(c.batch) * span.T * q_heads *
+                           splits * c.hdp;
   a.scale = scale * kLog2e;
   a.q_heads = q_heads;
   a.group = q_heads / c.kv_heads;
   const long long rows = static_cast<long long>(span.T) * a.group;
   const long long all = static_cast<long long>(c.batch) * span.T * q_heads;
-  const long long grid =
-      (rows + 15) / 16 * c.batch * c.kv_heads * splits;
-  if (rows > 0x7ffffff0LL || all > 0x7fffffffLL || grid > 0x7fffffffLL)
+  const int tile = tile_rows(rows, c.hdp);
+  const long long tiles = (rows + tile - 1) / tile;
+  const long long grid = tiles * c.batch * c.kv_heads * splits;
+  if (rows > 0x7fffff00LL || all > 0x7fffffffLL || grid > 0x7fffffffLL)
     return hipErrorInvalidValue;
   a.rows = static_cast<int>(rows);
-  a.tiles = static_cast<int>((rows + 15) / 16);
+  a.tiles = static_cast<int>(tiles);
   a.splits = splits;
   hipError_t err = hipSuccess;
-  FMA_BY_TYPE16(c.bf16, FMA_BY_BOOL(c.fp8, FP8, FMA_BY_WIDTH(c.hdp,
-      err = launch(kv8_attn_kernel<NS, FP8, E>,
-                   dim3(static_cast<unsigned>(grid)), 256, 0, stream, a))));
+  const dim3 g(static_cast<unsigned>(grid));
+  if (tile == 16) {
+    FMA_BY_TYPE16(c.bf16, FMA_BY_BOOL(c.fp8, FP8, FMA_BY_WIDTH(c.hdp,
+        err = launch(kv8_attn_few_kernel<NS, FP8, E>, g, 256, 0, stream, a))));
+  } else {
+    FMA_BY_TYPE16(c.bf16, FMA_BY_BOOL(c.fp8, FP8, FMA_BY_WIDTH(c.hdp,
+        err = launch(kv8_attn_many_kernel<NS, FP8, E, many_nr(NS)>, g, 256, 0,
+                     stream, a))));
+  }
   if (err != hipSuccess || splits == 1) return err;
-  const int threads = c.hd <= 64 ? 64 : c.hd <= 128 ? 128 : 256;
-  FMA_BY_TYPE16(c.bf16,
-      return launch(kv8_join_kernel<E>, dim3(static_cast<unsigned>(all)),
-                    threads, 0, stream, partials, static_cast<uint16_t*>(out),
-                    all, splits, c.hd, c.hdp));
+  FMA_BY_TYPE16(c.bf16, FMA_BY_WIDTH(c.hdp,
+      return launch(kv8_join_kernel<NS, E>, dim3(static_cast<unsigned>(all)),
+                    256, 0, stream, a.partials, a.stats,
+                    static_cast<uint16_t*>(out), splits, c.hd)));
 }
