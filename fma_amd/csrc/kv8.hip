@@ -704,7 +704,8 @@ struct AttnArgs {
   void* out;
   float* partials;  // [rows, splits, HDP]
   float* stats;     // [rows, splits, 2]: reference and sum
-  float scale;  // of the scores, times log2(e)
+  float scale;  // of the scores, its magnitude times log2(e)
+  int negative;
   int q_heads, group, rows, tiles, splits;
 };
 
@@ -734,6 +735,37 @@ __device__ inline float row_max(float x) {
   return fmaxf(x, __shfl_xor(x, 32));
 }
 
+// The running reference of V's scales. It moves where fp16 has no room for
+// the ratio to it; down only as far as fp32 sums cannot overflow.
+template <bool FP8>
+struct ScaleRef {
+  float ref = 0.0f, inv = 0.0f, most = 0.0f;
+  __device__ bool moves(float scale) const {
+    return !(scale <= ref * 64.0f) ||
+           (scale < ref * 0.015625f && scale >= most * 5.4e-20f);
+  }
+  // what to multiply outputs with
+  __device__ float move(float scale) {
+    const float f = ref != 0.0f ? ref / scale : 1.0f;
+    ref = scale;
+    inv = 1.0f / scale;
+    most = fmaxf(most, scale);
+    return f;
+  }
+  // scale / ref; between powers of two it is a difference of exponents
+  __device__ float ratio(float scale) const {
+    if constexpr (FP8)
+      return __int_as_float(max(
+          __float_as_int(scale) - __float_as_int(ref) + 0x3f800000, 0x800000));
+    else
+      return scale * inv;
+  }
+};
+
+// No score seen yet. Finite, so that a row that sees nothing needs no case of
+// its own: its weights are exp2(-inf) and its factors multiply zeros.
+constexpr float kNone = -3e38f;
+
 // One wave's softmax and output state for 16 query rows.
 template <int NS>
 struct RowState {
@@ -742,7 +774,7 @@ struct RowState {
   __device__ void clear() {
 #pragma unroll
     for (int n = 0; n < 2 * NS; ++n) o[n] = f32x4{0, 0, 0, 0};
-    m = -INFINITY;
+    m = kNone;
     l = 0.0f;
   }
   __device__ void times(float f) {
@@ -751,42 +783,79 @@ struct RowState {
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[n][r] *= f;
   }
-  // x: products of a block, f: what makes them log2 scores. On return the
-  // weights, with the sum advanced. The reference moves only when a score
-  // passes it by 2^8, which fp16 weights and fp32 sums have room for: the
-  // output is rarely rescaled, and while no lane asks for it, no value has to
-  // cross lanes.
-  template <bool MASK>
-  __device__ void weigh(f32x4 (&x)[2], float f, int left) {
+  __device__ void refer(float top, float more) {
+    top = row_max(top);
+    const float next = top > m + 8.0f ? top : m;
+    const float g = exp2f(m - next);
+    m = next;
+    l *= g;
+    times(g * more);
+  }
+};
+
+// x: products of a block with NR times 16 rows; f > 0: what makes them log2
+// scores; left: how many of the lane's tokens on are seen. On return x holds
+// the weights, and the sums are advanced. A row's reference moves only when a
+// score passes it by 2^8, which fp16 weights and fp32 sums have room for: the
+// outputs are rarely rescaled, and while no lane asks for it, no value has to
+// cross lanes.
+template <int NS, int NR, bool MASK, typename VS>
+__device__ inline void weigh(f32x4 (&x)[NR][2], const float (&f)[NR],
+                             const int (&left)[NR], RowState<NS> (&st)[NR],
+                             VS& vs, float vscale) {
+  float top[NR];
+  bool grows = false;
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+  for (int r = 0; r < NR; ++r) {
+    if (MASK) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x[a][r] *= f;
-        if (MASK && 16 * a + r >= left) x[a][r] = -INFINITY;
-      }
-    float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
-                      fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-    if (__any(top > m + 8.0f)) {
-      top = row_max(top);
-      const float next = top > m + 8.0f ? top : m;
-      const float g = next == m ? 1.0f : exp2f(m - next);
-      m = next;
-      l *= g;
-      times(g);
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (16 * a + i >= left[r]) x[r][a][i] = -INFINITY;
     }
-    const float ref = MASK && m == -INFINITY ? 0.0f : m;
+    top[r] = f[r] * fmaxf(fmaxf(fmaxf(x[r][0][0], x[r][0][1]),
+                                fmaxf(x[r][0][2], x[r][0][3])),
+                          fmaxf(fmaxf(x[r][1][0], x[r][1][1]),
+                                fmaxf(x[r][1][2], x[r][1][3])));
+    grows |= top[r] > st[r].m + 8.0f;
+  }
+  const bool moves = vs.moves(vscale);
+  if (__any(grows) || moves) {
+    const float more = moves ? vs.move(vscale) : 1.0f;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) st[r].refer(top[r], more);
+  }
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
     float sum = 0.0f;
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x[a][r] = __builtin_amdgcn_exp2f(x[a][r] - ref);
-        sum += x[a][r];
+      for (int i = 0; i < 4; ++i) {
+        x[r][a][i] =
+            __builtin_amdgcn_exp2f(fmaf(x[r][a][i], f[r], -st[r].m));
+        sum += x[r][a][i];
       }
-    l += sum;
+    st[r].l += sum;
   }
-};
+}
+// log2 scores of a block: K's scale times the row's factor, kept off zero and
+// infinity, which would make NaN of what is masked or zero
+__device__ inline float factor(float kscale, float qscale) {
+  return fminf(fmaxf(kscale * qscale, 1.2e-38f), 3e38f);
+}
+
+template <bool FP8>
+__device__ inline h8 weights16(const f32x4 (&x)[2], float ratio) {
+  h8 p;
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      p[4 * a + i] = static_cast<_Float16>(FP8 ? x[a][i] : x[a][i] * ratio);
+  return p;
+}
 
 // Where a tile of query rows reads its keys: its sequence, its blocks held as
 // codes, and whether it sees the incomplete block.
@@ -843,7 +912,8 @@ __device__ inline float query_fp16(const AttnArgs& A, const u16x8 (&raw)[NS],
   // 2^-e brings the row's largest into [2^9, 2^10)
   int e = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 9;
   e = top == 0.0f ? 0 : min(max(e, -100), 100);
-  const float mul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  const float size = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  const float mul = A.negative ? -size : size;
 #pragma unroll
   for (int ks = 0; ks < NS; ++ks)
 #pragma unroll
@@ -852,20 +922,9 @@ __device__ inline float query_fp16(const AttnArgs& A, const u16x8 (&raw)[NS],
   return A.scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 }
 
-// The running reference of V's scales. It moves where fp16 has no room for
-// the ratio to it; down only as far as fp32 sums cannot overflow.
-struct ScaleRef {
-  float ref, most;
-  // true: multiply the outputs by *f
-  __device__ bool move(float scale, float* f) {
-    if (scale <= ref * 64.0f &&
-        !(scale < ref * 0.015625f && scale >= most * 5.4e-20f))
-      return false;
-    *f = ref != 0.0f ? ref / scale : 1.0f;
-    ref = scale;
-    most = fmaxf(most, scale);
-    return true;
-  }
+struct NoScale {  // values that need none
+  __device__ bool moves(float) const { return false; }
+  __device__ float move(float) { return 1.0f; }
 };
 
 // The incomplete block, raw, for 16 rows. Its weights go in as two 16-bit
@@ -873,21 +932,30 @@ struct ScaleRef {
 template <int NS, typename E>
 __device__ inline void tail_step(const AttnArgs& A, const Reach& R, int bh,
                                  int lane, const u16x8 (&q)[NS], int seen,
-                                 RowState<NS>& st) {
+                                 RowState<NS> (&state)[1]) {
+  RowState<NS>& st = state[0];
   const int g = lane >> 4;
   const uint16_t* const kt =
       static_cast<const uint16_t*>(A.c.tail) +
       (static_cast<long long>(bh) * 2 + (R.full & 1)) * BLK * NS * 32 +
       lane * 16;
   const uint16_t* const vt = kt + A.c.tail_v;
-  f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  f32x4 xs[1][2] = {{{0, 0, 0, 0}, {0, 0, 0, 0}}};
+  f32x4(&x)[2] = xs[0];
 #pragma unroll
   for (int ks = 0; ks < NS; ++ks)
 #pragma unroll
     for (int a = 0; a < 2; ++a)
       x[a] = mfma16<E>(*reinterpret_cast<const u16x8*>(kt + ks * 1024 + a * 8),
                        q[ks], x[a]);
-  st.template weigh<true>(x, A.scale, seen - R.full * BLK - 4 * g);
+  if (A.negative) {
+    x[0] = -x[0];
+    x[1] = -x[1];
+  }
+  const float f[1] = {A.scale};
+  const int left[1] = {seen - R.full * BLK - 4 * g};
+  NoScale none;
+  weigh<NS, 1, true>(xs, f, left, state, none, 0.0f);
   u16x8 hi, lo;
 #pragma unroll
   for (int a = 0; a < 2; ++a)
@@ -933,16 +1001,17 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
   const bool live = row < A.rows && t < R.s.count;
   const int seen = live ? R.s.start + t + 1 : 0;  // keys of this row
 
-  RowState<NS> st;
+  RowState<NS> state[1];
+  RowState<NS>& st = state[0];
   st.clear();
 
   if (R.lo < R.hi || R.tail) {
     const uint16_t* const qrow = static_cast<const uint16_t*>(A.q.p) +
                                  b * A.q.sb + t * A.q.st + hq * A.q.sh;
-    u16x8 qraw[NS];
+    u16x8 raw[NS];
     h8 q[NS];
-    load_query<NS, E>(A, qrow, live, g, qraw);
-    const float qscale = query_fp16<NS, E>(A, qraw, q);
+    load_query<NS, E>(A, qrow, live, g, raw);
+    const float qscale = query_fp16<NS, E>(A, raw, q);
 
     const unsigned char* const kc =
         c.codes + static_cast<long long>(bh) * c.nblk * BLK * HDP + lane * 16;
@@ -950,8 +1019,9 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
     const float* const ksc = c.scales + static_cast<long long>(bh) * c.nblk;
     const float* const vsc = ksc + c.scales_v;
 
-    ScaleRef vs{0.0f, 0.0f};
+    ScaleRef<FP8> vs;
     u32x4 kr[NS], vr[NS];
+    float k_next = 0.0f, v_next = 0.0f;
     auto load = [&](int blk) {
       const long long at = static_cast<long long>(blk) * BLK * HDP;
 #pragma unroll
@@ -960,34 +1030,30 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
 #pragma unroll
       for (int i = 0; i < NS; ++i)
         vr[i] = *reinterpret_cast<const u32x4*>(vc + at + i * 1024);
+      k_next = ksc[blk];
+      v_next = vsc[blk];
     };
     int blk = R.lo + wave;
     if (blk < R.hi) load(blk);
     for (; blk < R.hi; blk += 4) {
-      const float kscale = ksc[blk], vscale = vsc[blk];
-      f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+      const float kscale = k_next, vscale = v_next;
+      f32x4 x[1][2] = {{{0, 0, 0, 0}, {0, 0, 0, 0}}};
 #pragma unroll
       for (int ks = 0; ks < NS; ++ks) {
-        x[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-            decode8(kr[ks][0], kr[ks][1], 1.0f, FP8), q[ks], x[0], 0, 0, 0);
-        x[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-            decode8(kr[ks][2], kr[ks][3], 1.0f, FP8), q[ks], x[1], 0, 0, 0);
+        x[0][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            decode8(kr[ks][0], kr[ks][1], 1.0f, FP8), q[ks], x[0][0], 0, 0, 0);
+        x[0][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            decode8(kr[ks][2], kr[ks][3], 1.0f, FP8), q[ks], x[0][1], 0, 0, 0);
       }
       u32x4 v_now[NS];
 #pragma unroll
       for (int i = 0; i < NS; ++i) v_now[i] = vr[i];
       if (blk + 4 < R.hi) load(blk + 4);
-      st.template weigh<true>(x, kscale * qscale, seen - blk * BLK - 4 * g);
-      float f;
-      if (vs.move(vscale, &f)) st.times(f);
-      const float ratio = vscale / vs.ref;
-      h8 p;
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          p[4 * a + r] =
-              static_cast<_Float16>(FP8 ? x[a][r] : x[a][r] * ratio);
+      const float f[1] = {factor(kscale, qscale)};
+      const int left[1] = {seen - blk * BLK - 4 * g};
+      weigh<NS, 1, true>(x, f, left, state, vs, vscale);
+      const float ratio = vs.ratio(vscale);
+      const h8 p = weights16<FP8>(x[0], ratio);
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         st.o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
@@ -999,7 +1065,10 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
       }
     }
     st.times(vs.ref);
-    if (R.tail && wave == 3) tail_step<NS, E>(A, R, bh, lane, qraw, seen, st);
+    if (R.tail && wave == 3) {
+      load_query<NS, E>(A, qrow, live, g, raw);
+      tail_step<NS, E>(A, R, bh, lane, raw, seen, state);
+    }
   }
 
   // join the four waves
@@ -1020,11 +1089,10 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
     if (orow >= A.rows) continue;
     const float m = fmaxf(fmaxf(s_m[0][rr], s_m[1][rr]),
                           fmaxf(s_m[2][rr], s_m[3][rr]));
-    const float ref = m == -INFINITY ? 0.0f : m;
     float o = 0.0f, sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float f = exp2f(s_m[w][rr] - ref);
+      const float f = exp2f(s_m[w][rr] - m);
       o += s_o[w][rr][d] * f;
       sum += s_l[w][rr] * f;
     }
@@ -1053,6 +1121,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
   constexpr int HDP = NS * 32;
   constexpr int UNITS = 2 * NS * 64;  // of 16 bytes in a block of K and V
   __shared__ u32x4 s_kv[2][UNITS];
+  __shared__ float s_scale[2][2];
   const FmaKv8Layer& c = A.c;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g = lane >> 4, n16 = lane & 15;
@@ -1102,6 +1171,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
     const float* const vsc = ksc + c.scales_v;
     constexpr int EACH = (UNITS + 255) / 256;
     u32x4 next[EACH];
+    float scale_next = 0.0f;
     auto load = [&](int blk) {
       const unsigned char* const at = kc + static_cast<long long>(blk) * BLK * HDP;
 #pragma unroll
@@ -1112,6 +1182,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
               at + (u < UNITS / 2 ? 0 : c.codes_v - BLK * HDP) +
               static_cast<long long>(u) * 16);
       }
+      if (threadIdx.x < 2) scale_next = (threadIdx.x ? vsc : ksc)[blk];
     };
     auto store = [&](int buf) {
 #pragma unroll
@@ -1119,15 +1190,18 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
         const int u = threadIdx.x + i * 256;
         if (UNITS % 256 == 0 || u < UNITS) s_kv[buf][u] = next[i];
       }
+      if (threadIdx.x < 2) s_scale[buf][threadIdx.x] = scale_next;
     };
     load(R.lo);
     store(0);
     __syncthreads();
-    ScaleRef vs{0.0f, 0.0f};
+    ScaleRef<FP8> vs;
     for (int blk = R.lo; blk < R.hi; ++blk) {
       const int buf = (blk - R.lo) & 1;
       if (blk + 1 < R.hi) load(blk + 1);
-      const float kscale = ksc[blk], vscale = vsc[blk];
+      const float kscale = s_scale[buf][0];
+      const float vscale = __uint_as_float(
+          __builtin_amdgcn_readfirstlane(__float_as_uint(s_scale[buf][1])));
       f32x4 x[NR][2];
 #pragma unroll
       for (int r = 0; r < NR; ++r)
@@ -1145,31 +1219,27 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
                                                            x[r][1], 0, 0, 0);
         }
       }
-      if (blk < clear) {
+      float f[NR];
+      int left[NR];
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        f[r] = factor(kscale, qscale[r]);
+        left[r] = seen[r] - blk * BLK - 4 * g;
+      }
+      if (blk >= clear) {
 #pragma unroll
         for (int r = 0; r < NR; ++r)
-          st[r].template weigh<false>(x[r], kscale * qscale[r], 0);
-      } else {
 #pragma unroll
-        for (int r = 0; r < NR; ++r)
-          st[r].template weigh<true>(x[r], kscale * qscale[r],
-                                     seen[r] - blk * BLK - 4 * g);
-      }
-      float f;
-      if (vs.move(vscale, &f)) {
+          for (int a = 0; a < 2; ++a)
 #pragma unroll
-        for (int r = 0; r < NR; ++r) st[r].times(f);
+            for (int i = 0; i < 4; ++i)
+              if (16 * a + i >= left[r]) x[r][a][i] = -INFINITY;
       }
-      const float ratio = vscale / vs.ref;
+      weigh<NS, NR, false>(x, f, left, st, vs, vscale);
+      const float ratio = vs.ratio(vscale);
       h8 p[NR];
 #pragma unroll
-      for (int r = 0; r < NR; ++r)
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            p[r][4 * a + i] =
-                static_cast<_Float16>(FP8 ? x[r][a][i] : x[r][a][i] * ratio);
+      for (int r = 0; r < NR; ++r) p[r] = weights16<FP8>(x[r], ratio);
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         const u32x4 w = s_kv[buf][(NS + i) * 64 + lane];
@@ -1194,7 +1264,8 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
     for (int r = 0; r < NR; ++r) {
       u16x8 raw[NS];
       load_query<NS, E>(A, qrow[r], live[r], g, raw);
-      tail_step<NS, E>(A, R, bh, lane, raw, seen[r], st[r]);
+      tail_step<NS, E>(A, R, bh, lane, raw, seen[r],
+                       *reinterpret_cast<RowState<NS>(*)[1]>(&st[r]));
     }
   }
 
@@ -1262,17 +1333,16 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(const float* partials,
     for (int i = 0; i < 2; ++i) {
       const int s = tid + 64 * i;
       const float* const st = stats + (row * splits + s) * 2;
-      m[i] = s < splits ? st[0] : -INFINITY;
+      m[i] = s < splits ? st[0] : kNone;
       l[i] = s < splits ? st[1] : 0.0f;
     }
     float top = fmaxf(m[0], m[1]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const float ref = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float w = exp2f(m[i] - ref);
+      const float w = exp2f(m[i] - top);
       s_w[tid + 64 * i] = w;
       sum += w * l[i];
     }
@@ -1440,7 +1510,8 @@ extern "C" hipError_t fma_launch_kv8_attention(FmaKv8Layer c, FmaKv8Span span,
   a.partials = partials;
   a.stats = partials + static_cast<long long>(c.batch) * span.T * q_heads *
                            splits * c.hdp;
-  a.scale = scale * kLog2e;
+  a.scale = fmaxf(fabsf(scale) * kLog2e, 1.2e-38f);
+  a.negative = scale < 0.0f;
   a.q_heads = q_heads;
   a.group = q_heads / c.kv_heads;
   const long long rows = static_cast<long long>(span.T) * a.group;
