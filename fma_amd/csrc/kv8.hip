@@ -740,12 +740,14 @@ __device__ inline float row_max(float x) {
 template <bool FP8>
 struct ScaleRef {
   float ref = 0.0f, inv = 0.0f, most = 0.0f;
-  __device__ bool moves(float scale) const {
-    return !(scale <= ref * 64.0f) ||
-           (scale < ref * 0.015625f && scale >= most * 5.4e-20f);
+  // a difference of bits is one of exponents, to a part of one
+  __device__ bool far(float scale) const {
+    return static_cast<uint32_t>(__float_as_int(scale) - __float_as_int(ref) +
+                                 (6 << 23)) > (12u << 23);
   }
-  // what to multiply outputs with
+  // moves it; returns what to multiply outputs with
   __device__ float move(float scale) {
+    if (scale < ref && !(scale >= most * 5.4e-20f)) return 1.0f;
     const float f = ref != 0.0f ? ref / scale : 1.0f;
     ref = scale;
     inv = 1.0f / scale;
@@ -814,15 +816,17 @@ __device__ inline void weigh(f32x4 (&x)[NR][2], const float (&f)[NR],
         for (int i = 0; i < 4; ++i)
           if (16 * a + i >= left[r]) x[r][a][i] = -INFINITY;
     }
-    top[r] = f[r] * fmaxf(fmaxf(fmaxf(x[r][0][0], x[r][0][1]),
-                                fmaxf(x[r][0][2], x[r][0][3])),
-                          fmaxf(fmaxf(x[r][1][0], x[r][1][1]),
-                                fmaxf(x[r][1][2], x[r][1][3])));
+    // v_maximum3: NaN comes through and moves nothing
+    float y = __builtin_elementwise_maximum(x[r][0][0], x[r][0][1]);
+#pragma unroll
+    for (int i = 2; i < 8; ++i)
+      y = __builtin_elementwise_maximum(y, x[r][i >> 2][i & 3]);
+    top[r] = f[r] * y;
     grows |= top[r] > st[r].m + 8.0f;
   }
-  const bool moves = vs.moves(vscale);
-  if (__any(grows) || moves) {
-    const float more = moves ? vs.move(vscale) : 1.0f;
+  const bool far = vs.far(vscale);
+  if (__any(grows) || far) {
+    const float more = far ? vs.move(vscale) : 1.0f;
 #pragma unroll
     for (int r = 0; r < NR; ++r) st[r].refer(top[r], more);
   }
@@ -923,7 +927,7 @@ __device__ inline float query_fp16(const AttnArgs& A, const u16x8 (&raw)[NS],
 }
 
 struct NoScale {  // values that need none
-  __device__ bool moves(float) const { return false; }
+  __device__ bool far(float) const { return false; }
   __device__ float move(float) { return 1.0f; }
 };
 
