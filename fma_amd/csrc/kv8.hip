@@ -745,9 +745,10 @@ struct ScaleRef {
     return static_cast<uint32_t>(__float_as_int(scale) - __float_as_int(ref) +
                                  (6 << 23)) > (12u << 23);
   }
-  // moves it; returns what to multiply outputs with
-  __device__ float move(float scale) {
-    if (scale < ref && !(scale >= most * 5.4e-20f)) return 1.0f;
+  // moves it where need be; returns what to multiply outputs with
+  __device__ float follow(float scale) {
+    if (!far(scale) || (scale < ref && !(scale >= most * 5.4e-20f)))
+      return 1.0f;
     const float f = ref != 0.0f ? ref / scale : 1.0f;
     ref = scale;
     inv = 1.0f / scale;
@@ -795,54 +796,56 @@ struct RowState {
   }
 };
 
-// x: products of a block with NR times 16 rows; f > 0: what makes them log2
-// scores; left: how many of the lane's tokens on are seen. On return x holds
-// the weights, and the sums are advanced. A row's reference moves only when a
-// score passes it by 2^8, which fp16 weights and fp32 sums have room for: the
-// outputs are rarely rescaled, and while no lane asks for it, no value has to
-// cross lanes.
-template <int NS, int NR, bool MASK, typename VS>
-__device__ inline void weigh(f32x4 (&x)[NR][2], const float (&f)[NR],
-                             const int (&left)[NR], RowState<NS> (&st)[NR],
-                             VS& vs, float vscale) {
+// x: products of NE blocks with NR times 16 rows; f > 0: what makes them log2
+// scores. A row's reference moves only when a score passes it by 2^8, which
+// fp16 weights and fp32 sums have room for: the outputs are rarely rescaled,
+// and while no lane asks for it, no value has to cross lanes.
+// more: what the outputs are to be multiplied with in any case.
+template <int NS, int NR, int NE>
+__device__ inline void settle(const f32x4 (&x)[NE][NR][2],
+                              const float (&f)[NE][NR], RowState<NS> (&st)[NR],
+                              float more) {
   float top[NR];
   bool grows = false;
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
-    if (MASK) {
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+    for (int e = 0; e < NE; ++e) {
+      // v_maximum3: NaN comes through and moves nothing
+      float y = __builtin_elementwise_maximum(x[e][r][0][0], x[e][r][0][1]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (16 * a + i >= left[r]) x[r][a][i] = -INFINITY;
+      for (int i = 2; i < 8; ++i)
+        y = __builtin_elementwise_maximum(y, x[e][r][i >> 2][i & 3]);
+      y *= f[e][r];
+      top[r] = e == 0 ? y : __builtin_elementwise_maximum(top[r], y);
     }
-    // v_maximum3: NaN comes through and moves nothing
-    float y = __builtin_elementwise_maximum(x[r][0][0], x[r][0][1]);
-#pragma unroll
-    for (int i = 2; i < 8; ++i)
-      y = __builtin_elementwise_maximum(y, x[r][i >> 2][i & 3]);
-    top[r] = f[r] * y;
     grows |= top[r] > st[r].m + 8.0f;
   }
-  const bool far = vs.far(vscale);
-  if (__any(grows) || far) {
-    const float more = far ? vs.move(vscale) : 1.0f;
+  if (__any(grows) || more != 1.0f) {
 #pragma unroll
     for (int r = 0; r < NR; ++r) st[r].refer(top[r], more);
   }
+}
+// x becomes the weights; their sum is advanced.
+template <int NS>
+__device__ inline void weigh(f32x4 (&x)[2], float f, RowState<NS>& st) {
+  float sum = 0.0f;
 #pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    float sum = 0.0f;
+  for (int a = 0; a < 2; ++a)
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int i = 0; i < 4; ++i) {
+      x[a][i] = __builtin_amdgcn_exp2f(fmaf(x[a][i], f, -st.m));
+      sum += x[a][i];
+    }
+  st.l += sum;
+}
+// left: how many of the lane's tokens on are seen
+__device__ inline void mask(f32x4 (&x)[2], int left) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[r][a][i] =
-            __builtin_amdgcn_exp2f(fmaf(x[r][a][i], f[r], -st[r].m));
-        sum += x[r][a][i];
-      }
-    st[r].l += sum;
-  }
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (16 * a + i >= left) x[a][i] = -INFINITY;
 }
 // log2 scores of a block: K's scale times the row's factor, kept off zero and
 // infinity, which would make NaN of what is masked or zero
@@ -926,11 +929,6 @@ __device__ inline float query_fp16(const AttnArgs& A, const u16x8 (&raw)[NS],
   return A.scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 }
 
-struct NoScale {  // values that need none
-  __device__ bool far(float) const { return false; }
-  __device__ float move(float) { return 1.0f; }
-};
-
 // The incomplete block, raw, for 16 rows. Its weights go in as two 16-bit
 // parts: a single bf16 would cost as much as the result's rounding.
 template <int NS, typename E>
@@ -944,8 +942,8 @@ __device__ inline void tail_step(const AttnArgs& A, const Reach& R, int bh,
       (static_cast<long long>(bh) * 2 + (R.full & 1)) * BLK * NS * 32 +
       lane * 16;
   const uint16_t* const vt = kt + A.c.tail_v;
-  f32x4 xs[1][2] = {{{0, 0, 0, 0}, {0, 0, 0, 0}}};
-  f32x4(&x)[2] = xs[0];
+  f32x4 xs[1][1][2] = {{{{0, 0, 0, 0}, {0, 0, 0, 0}}}};
+  f32x4(&x)[2] = xs[0][0];
 #pragma unroll
   for (int ks = 0; ks < NS; ++ks)
 #pragma unroll
@@ -956,10 +954,10 @@ __device__ inline void tail_step(const AttnArgs& A, const Reach& R, int bh,
     x[0] = -x[0];
     x[1] = -x[1];
   }
-  const float f[1] = {A.scale};
-  const int left[1] = {seen - R.full * BLK - 4 * g};
-  NoScale none;
-  weigh<NS, 1, true>(xs, f, left, state, none, 0.0f);
+  mask(x, seen - R.full * BLK - 4 * g);
+  const float f[1][1] = {{A.scale}};
+  settle<NS, 1, 1>(xs, f, state, 1.0f);
+  weigh<NS>(x, A.scale, st);
   u16x8 hi, lo;
 #pragma unroll
   for (int a = 0; a < 2; ++a)
@@ -1041,23 +1039,25 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
     if (blk < R.hi) load(blk);
     for (; blk < R.hi; blk += 4) {
       const float kscale = k_next, vscale = v_next;
-      f32x4 x[1][2] = {{{0, 0, 0, 0}, {0, 0, 0, 0}}};
+      f32x4 xs[1][1][2] = {{{{0, 0, 0, 0}, {0, 0, 0, 0}}}};
+      f32x4(&x)[2] = xs[0][0];
 #pragma unroll
       for (int ks = 0; ks < NS; ++ks) {
-        x[0][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-            decode8(kr[ks][0], kr[ks][1], 1.0f, FP8), q[ks], x[0][0], 0, 0, 0);
-        x[0][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-            decode8(kr[ks][2], kr[ks][3], 1.0f, FP8), q[ks], x[0][1], 0, 0, 0);
+        x[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            decode8(kr[ks][0], kr[ks][1], 1.0f, FP8), q[ks], x[0], 0, 0, 0);
+        x[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            decode8(kr[ks][2], kr[ks][3], 1.0f, FP8), q[ks], x[1], 0, 0, 0);
       }
       u32x4 v_now[NS];
 #pragma unroll
       for (int i = 0; i < NS; ++i) v_now[i] = vr[i];
       if (blk + 4 < R.hi) load(blk + 4);
-      const float f[1] = {factor(kscale, qscale)};
-      const int left[1] = {seen - blk * BLK - 4 * g};
-      weigh<NS, 1, true>(x, f, left, state, vs, vscale);
+      const float f[1][1] = {{factor(kscale, qscale)}};
+      mask(x, seen - blk * BLK - 4 * g);
+      settle<NS, 1, 1>(xs, f, state, vs.follow(vscale));
+      weigh<NS>(x, f[0][0], st);
       const float ratio = vs.ratio(vscale);
-      const h8 p = weights16<FP8>(x[0], ratio);
+      const h8 p = weights16<FP8>(x, ratio);
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         st.o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
@@ -1119,13 +1119,14 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
 }
 
 // Many rows: each of four waves has 16 * NR rows of its own, and all take the
-// same blocks, which go through LDS (two of them, one being filled).
-template <int NS, bool FP8, typename E, int NR>
+// same blocks, NE at a time, which go through LDS as fp16, so that each value
+// is decoded once for all of them; the next ones are on their way meanwhile.
+template <int NS, bool FP8, typename E, int NR, int NE>
 __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
   constexpr int HDP = NS * 32;
-  constexpr int UNITS = 2 * NS * 64;  // of 16 bytes in a block of K and V
-  __shared__ u32x4 s_kv[2][UNITS];
-  __shared__ float s_scale[2][2];
+  constexpr int UNITS = NS * 64;  // of 16 codes in a block of K or V
+  // a lane's operand of each 32 by 16 values, by lanes
+  __shared__ h8 s_k[2][NE][2 * NS][64], s_v[2][NE][2 * NS][64];
   const FmaKv8Layer& c = A.c;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g = lane >> 4, n16 = lane & 15;
@@ -1174,90 +1175,116 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
     const float* const ksc = c.scales + static_cast<long long>(bh) * c.nblk;
     const float* const vsc = ksc + c.scales_v;
     constexpr int EACH = (UNITS + 255) / 256;
-    u32x4 next[EACH];
+    const unsigned char* const vc = kc + c.codes_v;
+    // NE blocks of K and V, by way of registers. What lies behind the last
+    // block comes as zeros, with that block's scales. Lane e of each wave
+    // holds K's scale of block e, lane NE + e V's.
+    u32x4 kn[NE][EACH], vn[NE][EACH];
     float scale_next = 0.0f;
     auto load = [&](int blk) {
-      const unsigned char* const at = kc + static_cast<long long>(blk) * BLK * HDP;
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        const int u = threadIdx.x + i * 256;
-        if (UNITS % 256 == 0 || u < UNITS)
-          next[i] = *reinterpret_cast<const u32x4*>(
-              at + (u < UNITS / 2 ? 0 : c.codes_v - BLK * HDP) +
-              static_cast<long long>(u) * 16);
+      for (int e = 0; e < NE; ++e) {
+        const long long at = static_cast<long long>(blk + e) * BLK * HDP;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          const int u = threadIdx.x + i * 256;
+          kn[e][i] = vn[e][i] = u32x4{0, 0, 0, 0};
+          if ((UNITS % 256 == 0 || u < UNITS) && blk + e < R.hi) {
+            kn[e][i] = *reinterpret_cast<const u32x4*>(kc + at + u * 16);
+            vn[e][i] = *reinterpret_cast<const u32x4*>(vc + at + u * 16);
+          }
+        }
       }
-      if (threadIdx.x < 2) scale_next = (threadIdx.x ? vsc : ksc)[blk];
+      if (lane < 2 * NE)
+        scale_next = (lane < NE ? ksc : vsc)[min(blk + lane % NE, R.hi - 1)];
+    };
+    ScaleRef<FP8> vs;
+    // of the blocks in LDS: K's scale, what to multiply outputs with before
+    // them, and V's scale against the reference
+    float kscale[NE], more[NE], ratio[NE];
+    auto lane_of = [&](float x, int i) {
+      return __uint_as_float(
+          __builtin_amdgcn_readlane(__float_as_uint(x), i));
     };
     auto store = [&](int buf) {
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        const int u = threadIdx.x + i * 256;
-        if (UNITS % 256 == 0 || u < UNITS) s_kv[buf][u] = next[i];
+      for (int e = 0; e < NE; ++e) {
+        const float scale = lane_of(scale_next, NE + e);
+        kscale[e] = lane_of(scale_next, e);
+        more[e] = vs.follow(scale);
+        ratio[e] = vs.ratio(scale);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          const int u = threadIdx.x + i * 256;
+          if (UNITS % 256 == 0 || u < UNITS) {
+            const int n = 2 * (u >> 6), l = u & 63;
+            const u32x4 a = kn[e][i], w = vn[e][i];
+            s_k[buf][e][n][l] = decode8(a[0], a[1], 1.0f, FP8);
+            s_k[buf][e][n + 1][l] = decode8(a[2], a[3], 1.0f, FP8);
+            s_v[buf][e][n][l] = decode8(w[0], w[1], ratio[e], FP8);
+            s_v[buf][e][n + 1][l] = decode8(w[2], w[3], ratio[e], FP8);
+          }
+        }
       }
-      if (threadIdx.x < 2) s_scale[buf][threadIdx.x] = scale_next;
     };
     load(R.lo);
     store(0);
     __syncthreads();
-    ScaleRef<FP8> vs;
-    for (int blk = R.lo; blk < R.hi; ++blk) {
-      const int buf = (blk - R.lo) & 1;
-      if (blk + 1 < R.hi) load(blk + 1);
-      const float kscale = s_scale[buf][0];
-      const float vscale = __uint_as_float(
-          __builtin_amdgcn_readfirstlane(__float_as_uint(s_scale[buf][1])));
-      f32x4 x[NR][2];
+    for (int blk = R.lo; blk < R.hi; blk += NE) {
+      const int buf = ((blk - R.lo) / NE) & 1;
+      if (blk + NE < R.hi) load(blk + NE);
+      f32x4 x[NE][NR][2];
+      float f[NE][NR];
 #pragma unroll
-      for (int r = 0; r < NR; ++r)
-        x[r][0] = x[r][1] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int ks = 0; ks < NS; ++ks) {
-        const u32x4 w = s_kv[buf][ks * 64 + lane];
-        const h8 k0 = decode8(w[0], w[1], 1.0f, FP8);
-        const h8 k1 = decode8(w[2], w[3], 1.0f, FP8);
+      for (int e = 0; e < NE; ++e) {
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-          x[r][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[r][ks],
-                                                           x[r][0], 0, 0, 0);
-          x[r][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[r][ks],
-                                                           x[r][1], 0, 0, 0);
+          f[e][r] = factor(kscale[e], qscale[r]);
+          x[e][r][0] = x[e][r][1] = f32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int ks = 0; ks < NS; ++ks) {
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            const h8 kf = s_k[buf][e][2 * ks + a][lane];
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+              x[e][r][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  kf, q[r][ks], x[e][r][a], 0, 0, 0);
+          }
         }
       }
-      float f[NR];
-      int left[NR];
+      if (blk + NE > clear || blk + NE > R.hi) {
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        f[r] = factor(kscale, qscale[r]);
-        left[r] = seen[r] - blk * BLK - 4 * g;
+        for (int e = 0; e < NE; ++e)
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+            mask(x[e][r],
+                 blk + e < R.hi ? seen[r] - (blk + e) * BLK - 4 * g : 0);
       }
-      if (blk >= clear) {
+      settle<NS, NR, NE>(x, f, st, more[0]);
 #pragma unroll
-        for (int r = 0; r < NR; ++r)
+      for (int e = 0; e < NE; ++e) {
+        if (e > 0 && more[e] != 1.0f) {
 #pragma unroll
-          for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (16 * a + i >= left[r]) x[r][a][i] = -INFINITY;
-      }
-      weigh<NS, NR, false>(x, f, left, st, vs, vscale);
-      const float ratio = vs.ratio(vscale);
-      h8 p[NR];
-#pragma unroll
-      for (int r = 0; r < NR; ++r) p[r] = weights16<FP8>(x[r], ratio);
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const u32x4 w = s_kv[buf][(NS + i) * 64 + lane];
-        const h8 v0 = decode8(w[0], w[1], ratio, FP8);
-        const h8 v1 = decode8(w[2], w[3], ratio, FP8);
+          for (int r = 0; r < NR; ++r) st[r].times(more[e]);
+        }
+        h8 p[NR];
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-          st[r].o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              v0, p[r], st[r].o[2 * i], 0, 0, 0);
-          st[r].o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              v1, p[r], st[r].o[2 * i + 1], 0, 0, 0);
+          weigh<NS>(x[e][r], f[e][r], st[r]);
+          p[r] = weights16<FP8>(x[e][r], ratio[e]);
+        }
+#pragma unroll
+        for (int n = 0; n < 2 * NS; ++n) {
+          const h8 vf = s_v[buf][e][n][lane];
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+            st[r].o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                vf, p[r], st[r].o[n], 0, 0, 0);
         }
       }
-      if (blk + 1 < R.hi) store(buf ^ 1);
+      if (blk + NE < R.hi) store(buf ^ 1);
       __syncthreads();
     }
 #pragma unroll
@@ -1482,6 +1509,7 @@ namespace {
 // times NR.
 constexpr int kFewRows = 32;
 constexpr int many_nr(int ns) { return ns <= 4 ? 2 : 1; }
+constexpr int many_ne(int ns) { return ns <= 4 ? 2 : 1; }
 int tile_rows(long long rows, int hdp) {
   return rows <= kFewRows ? 16 : 64 * many_nr(hdp / 32);
 }
@@ -1535,8 +1563,8 @@ extern "C" hipError_t fma_launch_kv8_attention(FmaKv8Layer c, FmaKv8Span span,
         err = launch(kv8_attn_few_kernel<NS, FP8, E>, g, 256, 0, stream, a))));
   } else {
     FMA_BY_TYPE16(c.bf16, FMA_BY_BOOL(c.fp8, FP8, FMA_BY_WIDTH(c.hdp,
-        err = launch(kv8_attn_many_kernel<NS, FP8, E, many_nr(NS)>, g, 256, 0,
-                     stream, a))));
+        err = launch(kv8_attn_many_kernel<NS, FP8, E, many_nr(NS), many_ne(NS)>,
+                     g, 256, 0, stream, a))));
   }
   if (err != hipSuccess || splits == 1) return err;
   FMA_BY_TYPE16(c.bf16, FMA_BY_WIDTH(c.hdp,
