@@ -81,7 +81,15 @@ __device__ inline void load8(const typename E::raw* row, int d0, int hd,
     x[j] = d0 + j < hd ? E::to_f(row[d0 + j]) : 0.0f;
 }
 
-template <typename E>
+// PAST: past the caches, for outputs larger than they are.
+template <bool PAST, typename V>
+__device__ inline void put(void* at, V v) {
+  if constexpr (PAST)
+    __builtin_nontemporal_store(v, static_cast<V*>(at));
+  else
+    *static_cast<V*>(at) = v;
+}
+template <typename E, bool PAST>
 __device__ inline void store8(typename E::raw* row, int d0, int hd, bool vec,
                               const float (&x)[8]) {
   if (d0 >= hd) return;
@@ -90,13 +98,13 @@ __device__ inline void store8(typename E::raw* row, int d0, int hd, bool vec,
       u16x8 u;
 #pragma unroll
       for (int j = 0; j < 8; ++j) u[j] = E::from_f(x[j]);
-      *reinterpret_cast<u16x8*>(row + d0) = u;
+      put<PAST>(row + d0, u);
       return;
     }
   } else {
     if (vec) {
-      *reinterpret_cast<f32x4*>(row + d0) = f32x4{x[0], x[1], x[2], x[3]};
-      *reinterpret_cast<f32x4*>(row + d0 + 4) = f32x4{x[4], x[5], x[6], x[7]};
+      put<PAST>(row + d0, f32x4{x[0], x[1], x[2], x[3]});
+      put<PAST>(row + d0 + 4, f32x4{x[4], x[5], x[6], x[7]});
       return;
     }
   }
@@ -189,6 +197,15 @@ struct Turn {
           x[2 * j + 1] = fmaf(a, s[j], b * c[j]);
         }
       }
+    } else if ((r.half & 7) == 0) {
+      // the partners of a lane's values are one other lane's
+      const int by = r.half >> 3, li = d0 >> 3;
+      const int from = (threadIdx.x & 63) + (li < by ? by : -by);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float y = __shfl(x[j], from);
+        if (d0 < 2 * r.half) x[j] = fmaf(x[j], c[j], y * s[j]);
+      }
     } else {
       // value d of the row lies at [d % 8][d / 8]: neighbouring lanes on
       // neighbouring banks
@@ -223,37 +240,29 @@ __device__ inline long long pos_of(const FmaPos& p, int b, int t) {
   return p.per_token ? v : v + t;
 }
 
-// Heads [h0, h1) of one token, four rows in flight.
-template <typename E, int LPR, bool PAIRS>
+// Heads [h0, h1) of one token, one after the other: at 8192 tokens of 32 + 8
+// heads four in flight took 37.8 us, one 34.7 us, for more waves fit a CU.
+template <typename E, int LPR, bool PAIRS, bool PAST>
 __device__ inline void turn_heads(const Turn<LPR, PAIRS>& turn,
                                   const FmaRope& r, const FmaRows& in,
                                   long long base, typename E::raw* out, int h0,
                                   int h1, int hd, int d0, bool out_vec,
                                   bool zero, float* scratch) {
   const typename E::raw* src = static_cast<const typename E::raw*>(in.p) + base;
-  for (int h = h0; h < h1; h += 4) {
-    float x[4][8];
+  for (int h = h0; h < h1; ++h) {
+    float x[8];
+    load8<E>(src + h * in.sh, d0, hd, in.vec != 0, x);
+    turn.run(x, r, hd, d0, scratch);
+    if (zero) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (h + u < h1)
-        load8<E>(src + (h + u) * in.sh, d0, hd, in.vec != 0, x[u]);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (h + u < h1) {
-        turn.run(x[u], r, hd, d0, scratch);
-        if (zero) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[u][j] = 0.0f;
-        }
-        store8<E>(out + static_cast<long long>(h + u) * hd, d0, hd, out_vec,
-                  x[u]);
-      }
+      for (int j = 0; j < 8; ++j) x[j] = 0.0f;
     }
+    store8<E, PAST>(out + static_cast<long long>(h) * hd, d0, hd, out_vec, x);
   }
 }
 
 // A row of LPR lanes takes `per` heads of one token.
-template <typename E, int LPR, bool PAIRS>
+template <typename E, int LPR, bool PAIRS, bool PAST>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(
     FmaRows q, FmaRows k, void* qo, void* ko, int B, int T, int q_heads,
     int kv_heads, int hd, FmaRope r, FmaPos pos, int per, int q_items,
@@ -276,9 +285,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(
   Turn<LPR, PAIRS> turn;
   turn.at(r, pos_of(pos, b, t), d0);
   turn.template weights<E>(is_q ? r.qw : r.kw, d0, hd);
-  turn_heads<E, LPR, PAIRS>(turn, r, in, b * in.sb + t * in.st, out, h0, h1,
-                            hd, d0, hd % 8 == 0, false,
-                            scratch + (threadIdx.x / LPR) * LPR * 8);
+  turn_heads<E, LPR, PAIRS, PAST>(turn, r, in, b * in.sb + t * in.st, out, h0,
+                                  h1, hd, d0, hd % 8 == 0, false,
+                                  scratch + (threadIdx.x / LPR) * LPR * 8);
 }
 
 // ---------------------------------------------------------------------------
@@ -323,22 +332,16 @@ __device__ inline Span span_of(const FmaKv8Span& s, int b, int max_seq) {
 // last two blocks are also kept raw. Codes are made from the 16-bit values
 // only, so they do not depend on how tokens were spread over calls.
 
-template <typename E>
-__device__ inline bool is_finite16(uint16_t u) {
-  return (u & 0x7fffu) < E::kInf;
-}
-
 // 16 values -> 16 codes. NaN is 0, an infinity the block's largest value.
 template <typename E, bool FP8>
 __device__ inline u32x4 encode16(const uint16_t (&u)[16], float amax,
                                  float mul) {
+  const float top = amax * mul;
   float x[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    float f = E::to_f(u[i]);
-    const uint32_t m = u[i] & 0x7fffu;
-    if (m >= E::kInf) f = m > E::kInf ? 0.0f : copysignf(amax, f);
-    x[i] = f * mul;
+    const float f = E::to_f(u[i]);
+    x[i] = f == f ? fminf(fmaxf(f * mul, -top), top) : 0.0f;
   }
   u32x4 o;
 #pragma unroll
@@ -350,10 +353,9 @@ __device__ inline u32x4 encode16(const uint16_t (&u)[16], float amax,
     } else {
       uint32_t w = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float c = fminf(fmaxf(rintf(x[4 * i + j]), -127.0f), 127.0f);
-        w |= static_cast<uint32_t>(static_cast<int>(c) + 128) << (8 * j);
-      }
+      for (int j = 0; j < 4; ++j)
+        w |= static_cast<uint32_t>(static_cast<int>(rintf(x[4 * i + j])) + 128)
+             << (8 * j);
       o[i] = w;
     }
   }
@@ -379,7 +381,7 @@ __device__ inline void scale_of(float amax, float* scale, float* mul) {
   }
 }
 
-template <typename E, int LPR, bool PAIRS, bool FP8>
+template <typename E, int LPR, bool PAIRS, bool FP8, bool PAST>
 __global__ __launch_bounds__(256) void kv8_append_kernel(
     FmaKv8Layer c, FmaKv8Span sp, FmaRows q, FmaRows k, FmaRows v, void* qo,
     int q_heads, FmaRope r, int blocks, int kv_groups, int per, int q_items) {
@@ -407,7 +409,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(
     Turn<LPR, PAIRS> turn;
     turn.at(r, s.start + t < c.max_seq ? s.start + t : 0, d0);
     turn.template weights<E>(r.qw, d0, hd);
-    turn_heads<E, LPR, PAIRS>(
+    turn_heads<E, LPR, PAIRS, PAST>(
         turn, r, q, b * q.sb + t * q.st,
         static_cast<uint16_t*>(qo) + bt * q_heads * hd, item * per,
         min((item + 1) * per, q_heads), hd, d0, hd % 8 == 0, t >= s.count,
@@ -415,9 +417,11 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(
     return;
   }
 
-  const int j = blockIdx.x % blocks;
-  const int bh = blockIdx.x / blocks;
-  const int b = bh / c.kv_heads, h = bh - b * c.kv_heads;
+  // the heads of a block next to each other: their rows are
+  const int h = blockIdx.x % c.kv_heads;
+  const int bj = blockIdx.x / c.kv_heads;
+  const int b = bj / blocks, j = bj - b * blocks;
+  const int bh = b * c.kv_heads + h;
   const Span s = span_of(sp, b, c.max_seq);
   const int b0 = s.start / BLK, blk = b0 + j;
   if (s.count == 0 || blk * BLK >= s.end) return;
@@ -430,27 +434,47 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(
            (static_cast<long long>(bh) * 2 + (block & 1)) * BLK * c.hdp;
   };
 
+  uint32_t top[2] = {0, 0};  // largest finite magnitude, as bits
+  auto note = [&](int w, u16x8 u) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t m = u[e] & 0x7fffu;
+      top[w] = max(top[w], m < E::kInf ? m : 0u);
+    }
+  };
   // new tokens [lo, hi) of a block, into LDS
   auto fetch = [&](int block, int lo, int hi) {
+    constexpr int TURNS = BLK / ROWS;
+    float x[TURNS][8], y[TURNS][8];
+#pragma unroll
+    for (int n = 0; n < TURNS; ++n) {
+      const int i = n * ROWS + row, t = block * BLK + i - s.start;
+      if (block * BLK + i >= lo && block * BLK + i < hi) {
+        load8<E>(static_cast<const uint16_t*>(k.p) + b * k.sb + t * k.st +
+                     h * k.sh, d0, hd, k.vec != 0, x[n]);
+        load8<E>(static_cast<const uint16_t*>(v.p) + b * v.sb + t * v.st +
+                     h * v.sh, d0, hd, v.vec != 0, y[n]);
+      }
+    }
     Turn<LPR, PAIRS> turn;
     turn.template weights<E>(r.kw, d0, hd);
-    for (int i = lo - block * BLK + row; i < hi - block * BLK; i += ROWS) {
-      const int t = block * BLK + i - s.start;
-      float x[8], y[8];
-      load8<E>(static_cast<const uint16_t*>(k.p) + b * k.sb + t * k.st +
-                   h * k.sh, d0, hd, k.vec != 0, x);
-      load8<E>(static_cast<const uint16_t*>(v.p) + b * v.sb + t * v.st +
-                   h * v.sh, d0, hd, v.vec != 0, y);
-      turn.at(r, block * BLK + i, d0);
-      turn.run(x, r, hd, d0, my_scratch);
-      u16x8 xu, yu;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        xu[e] = d0 + e < hd ? E::from_f(x[e]) : 0;
-        yu[e] = E::from_f(y[e]);
+    for (int n = 0; n < TURNS; ++n) {
+      const int i = n * ROWS + row;
+      if (block * BLK + i >= lo && block * BLK + i < hi) {
+        turn.at(r, block * BLK + i, d0);
+        turn.run(x[n], r, hd, d0, my_scratch);
+        u16x8 xu, yu;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          xu[e] = d0 + e < hd ? E::from_f(x[n][e]) : 0;
+          yu[e] = E::from_f(y[n][e]);
+        }
+        note(0, xu);
+        note(1, yu);
+        *reinterpret_cast<u16x8*>(&tile[0][i][d0]) = xu;
+        *reinterpret_cast<u16x8*>(&tile[1][i][d0]) = yu;
       }
-      *reinterpret_cast<u16x8*>(&tile[0][i][d0]) = xu;
-      *reinterpret_cast<u16x8*>(&tile[1][i][d0]) = yu;
     }
   };
   // tokens [lo, hi) of a block from LDS to its raw slot
@@ -476,31 +500,18 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(
     const uint16_t* const vt = tail_at(1, blk);
     for (int i = row; i < lo - blk * BLK; i += ROWS) {
       if (d0 < c.hdp) {
-        *reinterpret_cast<u16x8*>(&tile[0][i][d0]) =
-            *reinterpret_cast<const u16x8*>(kt + kidx(i, d0));
+        const u16x8 x = *reinterpret_cast<const u16x8*>(kt + kidx(i, d0));
+        u16x8 y;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) tile[1][i][d0 + e] = vt[vidx(i, d0 + e)];
+        for (int e = 0; e < 8; ++e) y[e] = vt[vidx(i, d0 + e)];
+        note(0, x);
+        note(1, y);
+        *reinterpret_cast<u16x8*>(&tile[0][i][d0]) = x;
+        *reinterpret_cast<u16x8*>(&tile[1][i][d0]) = y;
       }
     }
   }
-  __syncthreads();
-
   if (complete) {
-    const int units = c.hdp * 2;  // of 16 values, for each of K and V
-    uint32_t top[2] = {0, 0};
-    for (int i = tid; i < BLK * LPR; i += 256) {
-      const int tok = i / LPR, d = (i % LPR) * 8;
-      if (d < c.hdp) {
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const u16x8 u = *reinterpret_cast<const u16x8*>(&tile[w][tok][d]);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (is_finite16<E>(u[e]))
-              top[w] = max(top[w], static_cast<uint32_t>(u[e] & 0x7fffu));
-        }
-      }
-    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
       top[0] = max(top[0], static_cast<uint32_t>(__shfl_xor(top[0], o)));
@@ -510,7 +521,11 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(
       s_max[0][tid >> 6] = top[0];
       s_max[1][tid >> 6] = top[1];
     }
-    __syncthreads();
+  }
+  __syncthreads();
+
+  if (complete) {
+    const int units = c.hdp * 2;  // of 16 values, for each of K and V
     float amax[2], mul[2];
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
@@ -1405,6 +1420,17 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(const float* partials,
   }
 }
 
+// Heads that a row of lanes takes: as many as leave every CU six workgroups
+// of 256 threads, at most 16 (8192 tokens of 32 + 8 heads: 4 heads 38.6 us, 8
+// 34.7 us, 16 31.7 us, 32 37.9 us).
+int heads_each(long long rows) {
+  const long long n = rows / (256 * 6 * 16);
+  return n < 1 ? 1 : n > 16 ? 16 : static_cast<int>(n);
+}
+// Outputs beyond the 32 MB of second-level caches are stored past them: at
+// 84 MB 37.8 us against 50.7 us.
+bool past_caches(long long bytes) { return bytes > (32LL << 20); }
+
 int lanes_per_row(int hd) { return hd <= 64 ? 8 : hd <= 128 ? 16 : 32; }
 
 template <typename... P, typename... Given>
@@ -1450,17 +1476,19 @@ extern "C" hipError_t fma_launch_qk_norm_rope(
     hipStream_t stream) {
   const long long tokens = static_cast<long long>(B) * T;
   if (tokens == 0) return hipSuccess;
-  const int per = tokens * (q_heads + kv_heads) < 8192 ? 1 : 8;
+  const int per = heads_each(tokens * (q_heads + kv_heads));
   const int q_items = (q_heads + per - 1) / per;
   const int items = q_items + (kv_heads + per - 1) / per;
   const int rows = 256 / lanes_per_row(hd);
   const long long grid = (tokens * items + rows - 1) / rows;
   if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
   FMA_BY_TYPE(type, FMA_BY_LANES(hd, FMA_BY_BOOL(rope.pairs, PAIRS,
-      return launch(qk_norm_rope_kernel<E, LPR, PAIRS>,
-                    dim3(static_cast<unsigned>(grid)), 256, 0, stream, q, k,
-                    qo, ko, B, T, q_heads, kv_heads, hd, rope, pos, per,
-                    q_items, items))));
+      FMA_BY_BOOL(past_caches(tokens * (q_heads + kv_heads) * hd *
+                              (type == 2 ? 4 : 2)), PAST,
+          return launch(qk_norm_rope_kernel<E, LPR, PAIRS, PAST>,
+                        dim3(static_cast<unsigned>(grid)), 256, 0, stream, q,
+                        k, qo, ko, B, T, q_heads, kv_heads, hd, rope, pos, per,
+                        q_items, items)))));
 }
 
 extern "C" hipError_t fma_launch_kv8_append(FmaKv8Layer c, FmaKv8Span span,
@@ -1474,7 +1502,7 @@ extern "C" hipError_t fma_launch_kv8_append(FmaKv8Layer c, FmaKv8Span span,
     blocks = (span.start_i + span.T - 1) / BLK - span.start_i / BLK + 1;
   const long long kv_groups =
       static_cast<long long>(c.batch) * c.kv_heads * blocks;
-  const int per = tokens * q_heads < 8192 ? 1 : 8;
+  const int per = heads_each(tokens * q_heads);
   const int q_items = (q_heads + per - 1) / per;
   const int rows = 256 / lanes_per_row(c.hd);
   const long long q_groups =
@@ -1483,9 +1511,11 @@ extern "C" hipError_t fma_launch_kv8_append(FmaKv8Layer c, FmaKv8Span span,
   const unsigned grid = static_cast<unsigned>(kv_groups + q_groups);
   FMA_BY_TYPE16(c.bf16, FMA_BY_LANES(c.hd, FMA_BY_BOOL(rope.pairs, PAIRS,
       FMA_BY_BOOL(c.fp8, FP8,
-          return launch(kv8_append_kernel<E, LPR, PAIRS, FP8>, dim3(grid), 256,
-                        0, stream, c, span, q, k, v, qo, q_heads, rope, blocks,
-                        static_cast<int>(kv_groups), per, q_items)))));
+          FMA_BY_BOOL(past_caches(tokens * q_heads * c.hd * 2), PAST,
+              return launch(kv8_append_kernel<E, LPR, PAIRS, FP8, PAST>,
+                            dim3(grid), 256, 0, stream, c, span, q, k, v, qo,
+                            q_heads, rope, blocks, static_cast<int>(kv_groups),
+                            per, q_items))))));
 }
 
 extern "C" hipError_t fma_launch_kv8_read(FmaKv8Layer c, const int* start,
