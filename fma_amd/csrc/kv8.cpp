@@ -2,9 +2,10 @@
 // kernels (kv8.hip). Every call checks what its kernel's grid and indexes
 // assume, runs on the current stream of the tensors' device, and takes its
 // workspace from the caching allocator, so calls on several streams and
-// captured graphs share nothing.
+// captured graphs share nothing. A call that does not fit is a ValueError.
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -25,12 +26,16 @@ int compute_units(int device) {
   return at::cuda::getDeviceProperties(device)->multiProcessorCount;
 }
 
-// [B, T, H, hd] with a contiguous last dimension.
-FmaRows rows_of(const at::Tensor& x, const char* name) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 4, name,
-              " must be a GPU tensor [B, T, heads, head_dim]");
-  TORCH_CHECK(x.size(3) == 1 || x.stride(3) == 1, name,
-              " needs a contiguous last dimension");
+// [B, T, H, hd], copied if its last dimension is not contiguous.
+at::Tensor dense_last(const at::Tensor& x, const char* name) {
+  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() == 4, name,
+                    " must be a GPU tensor [B, T, heads, head_dim]");
+  TORCH_CHECK_VALUE(!(x.requires_grad() && at::GradMode::is_enabled()), name,
+                    " requires a gradient; there is no backward pass");
+  return x.size(3) == 1 || x.stride(3) == 1 ? x : x.contiguous();
+}
+
+FmaRows rows_of(const at::Tensor& x) {
   FmaRows r;
   r.p = x.data_ptr();
   r.sb = x.stride(0);
@@ -47,7 +52,7 @@ FmaRows rows_of(const at::Tensor& x, const char* name) {
 }
 
 int type_of(at::ScalarType t) {
-  TORCH_CHECK(t == at::kBFloat16 || t == at::kHalf || t == at::kFloat,
+  TORCH_CHECK_VALUE(t == at::kBFloat16 || t == at::kHalf || t == at::kFloat,
               "bfloat16, float16 or float32 wanted, got ", t);
   return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : 2;
 }
@@ -60,18 +65,18 @@ FmaRope rope_of(const c10::optional<at::Tensor>& cos,
   FmaRope r{};
   r.eps = static_cast<float>(eps);
   r.pairs = pairs;
-  TORCH_CHECK(cos.has_value() == sin.has_value(), "cos and sin go together");
+  TORCH_CHECK_VALUE(cos.has_value() == sin.has_value(), "cos and sin go together");
   if (cos.has_value()) {
     const auto &c = *cos, &s = *sin;
-    TORCH_CHECK(c.device() == like.device() && s.device() == like.device() &&
+    TORCH_CHECK_VALUE(c.device() == like.device() && s.device() == like.device() &&
                     c.scalar_type() == at::kFloat &&
                     s.scalar_type() == at::kFloat && c.dim() == 2 &&
                     c.sizes() == s.sizes() && c.is_contiguous() &&
                     s.is_contiguous(),
                 "cos/sin tables must be contiguous fp32 [S, rot/2] beside q");
-    TORCH_CHECK(c.size(1) >= 1 && 2 * c.size(1) <= hd,
+    TORCH_CHECK_VALUE(c.size(1) >= 1 && 2 * c.size(1) <= hd,
                 "the tables rotate more than head_dim");
-    TORCH_CHECK(c.size(0) >= 1 && c.size(0) <= 0x7fffffff, "bad table length");
+    TORCH_CHECK_VALUE(c.size(0) >= 1 && c.size(0) <= 0x7fffffff, "bad table length");
     r.cos = c.data_ptr<float>();
     r.sin = s.data_ptr<float>();
     r.half = static_cast<int>(c.size(1));
@@ -79,7 +84,7 @@ FmaRope rope_of(const c10::optional<at::Tensor>& cos,
   }
   auto weight = [&](const c10::optional<at::Tensor>& w) -> const void* {
     if (!w.has_value()) return nullptr;
-    TORCH_CHECK(w->device() == like.device() &&
+    TORCH_CHECK_VALUE(w->device() == like.device() &&
                     w->scalar_type() == like.scalar_type() &&
                     w->numel() == hd && w->is_contiguous(),
                 "norm weights must be contiguous [head_dim] of q's type");
@@ -91,29 +96,33 @@ FmaRope rope_of(const c10::optional<at::Tensor>& cos,
 }
 
 std::tuple<at::Tensor, at::Tensor> qk_norm_rope(
-    const at::Tensor& q, const at::Tensor& k, const at::Tensor& cos,
+    const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& cos,
     const at::Tensor& sin, const c10::optional<at::Tensor>& pos,
     int64_t start, const c10::optional<at::Tensor>& qw,
     const c10::optional<at::Tensor>& kw, double eps, bool pairs) {
-  const FmaRows qr = rows_of(q, "q"), kr = rows_of(k, "k");
+  const at::Tensor q = dense_last(q_in, "q"), k = dense_last(k_in, "k");
+  const FmaRows qr = rows_of(q), kr = rows_of(k);
   const int64_t B = q.size(0), T = q.size(1), hd = q.size(3);
-  TORCH_CHECK(k.device() == q.device() && k.scalar_type() == q.scalar_type() &&
+  TORCH_CHECK_VALUE(k.device() == q.device() && k.scalar_type() == q.scalar_type() &&
                   k.size(0) == B && k.size(1) == T && k.size(3) == hd,
               "k must match q but for the number of heads");
-  TORCH_CHECK(hd >= 2 && hd <= 256, "head_dim must be 2..256, got ", hd);
-  TORCH_CHECK(q.size(2) >= 1 && k.size(2) >= 1 && q.size(2) < (1 << 20) &&
+  TORCH_CHECK_VALUE(hd >= 2 && hd <= 256, "head_dim must be 2..256, got ", hd);
+  TORCH_CHECK_VALUE(q.size(2) >= 1 && k.size(2) >= 1 && q.size(2) < (1 << 20) &&
                   k.size(2) < (1 << 20) && B < (1 << 30) && T < (1 << 30),
               "bad shape");
   const int type = type_of(q.scalar_type());
   const FmaRope rope = rope_of(cos, sin, qw, kw, eps, pairs, q, hd);
   FmaPos p{};
   p.start = start;
+  TORCH_CHECK_VALUE(pos.has_value() || (start >= 0 && start + T <= rope.table),
+                    "positions [", start, ", ", start + T,
+                    ") lie outside the tables' ", rope.table);
   if (pos.has_value()) {
     const auto& t = *pos;
-    TORCH_CHECK(t.device() == q.device() && (t.scalar_type() == at::kInt ||
+    TORCH_CHECK_VALUE(t.device() == q.device() && (t.scalar_type() == at::kInt ||
                                              t.scalar_type() == at::kLong),
                 "positions must be int32 or int64 beside q");
-    TORCH_CHECK((t.dim() == 1 && t.size(0) == B) ||
+    TORCH_CHECK_VALUE((t.dim() == 1 && t.size(0) == B) ||
                     (t.dim() == 2 && t.size(0) == B && t.size(1) == T),
                 "positions must be [B] or [B, T]");
     if (t.scalar_type() == at::kInt)
@@ -143,29 +152,29 @@ class Kv8Buffers {
              int64_t max_seq, int64_t hd, bool fp8)
       : codes_(std::move(codes)), scales_(std::move(scales)),
         tail_(std::move(tail)) {
-    TORCH_CHECK(codes_.is_cuda() && codes_.scalar_type() == at::kByte &&
+    TORCH_CHECK_VALUE(codes_.is_cuda() && codes_.scalar_type() == at::kByte &&
                     codes_.dim() == 6 && codes_.is_contiguous(),
                 "codes must be uint8 [L, 2, B, kvH, blocks, 32 * width]");
     layers_ = codes_.size(0);
     const int64_t B = codes_.size(2), H = codes_.size(3), n = codes_.size(4);
     const int64_t width = codes_.size(5) / FMA_KV8_BLOCK;
-    TORCH_CHECK(codes_.size(1) == 2 && layers_ >= 1 && B >= 1 && H >= 1 &&
+    TORCH_CHECK_VALUE(codes_.size(1) == 2 && layers_ >= 1 && B >= 1 && H >= 1 &&
                     n >= 1 && codes_.size(5) % FMA_KV8_BLOCK == 0,
                 "bad shape of codes");
-    TORCH_CHECK(width == 32 || width == 64 || width == 96 || width == 128 ||
+    TORCH_CHECK_VALUE(width == 32 || width == 64 || width == 96 || width == 128 ||
                     width == 192 || width == 256,
                 "unsupported width ", width);
-    TORCH_CHECK(hd >= 1 && hd <= width, "head_dim beyond the width");
-    TORCH_CHECK(max_seq >= 1 && max_seq <= n * FMA_KV8_BLOCK &&
+    TORCH_CHECK_VALUE(hd >= 1 && hd <= width, "head_dim beyond the width");
+    TORCH_CHECK_VALUE(max_seq >= 1 && max_seq <= n * FMA_KV8_BLOCK &&
                     max_seq < (1 << 30),
                 "max_seq beyond the blocks");
-    TORCH_CHECK(B * H < (1 << 30), "too many sequences");
-    TORCH_CHECK(scales_.device() == codes_.device() &&
+    TORCH_CHECK_VALUE(B * H < (1 << 30), "too many sequences");
+    TORCH_CHECK_VALUE(scales_.device() == codes_.device() &&
                     scales_.scalar_type() == at::kFloat &&
                     scales_.is_contiguous() &&
                     scales_.sizes() == at::IntArrayRef({layers_, 2, B, H, n}),
                 "scales must be fp32 [L, 2, B, kvH, blocks]");
-    TORCH_CHECK(tail_.device() == codes_.device() && tail_.is_contiguous() &&
+    TORCH_CHECK_VALUE(tail_.device() == codes_.device() && tail_.is_contiguous() &&
                     (tail_.scalar_type() == at::kBFloat16 ||
                      tail_.scalar_type() == at::kHalf) &&
                     tail_.sizes() ==
@@ -187,7 +196,9 @@ class Kv8Buffers {
   void append(int64_t layer, const at::Tensor& k, const at::Tensor& v,
               const c10::optional<at::Tensor>& start, int64_t start_i,
               const c10::optional<at::Tensor>& counts) {
-    store(layer, nullptr, k, v, FmaRope{}, start, start_i, counts);
+    FmaRope none{};
+    none.pairs = 1;  // the lighter of the two kernels
+    store(layer, nullptr, k, v, none, start, start_i, counts);
   }
 
   at::Tensor norm_rope_append(
@@ -198,16 +209,17 @@ class Kv8Buffers {
       const c10::optional<at::Tensor>& kw,
       const c10::optional<at::Tensor>& counts, double eps, bool pairs) {
     const FmaRope rope = rope_of(cos, sin, qw, kw, eps, pairs, tail_, c_.hd);
-    TORCH_CHECK(rope.table >= c_.max_seq,
+    TORCH_CHECK_VALUE(rope.table >= c_.max_seq,
                 "the cos/sin tables are shorter than the cache");
-    return store(layer, &q, k, v, rope, start, start_i, counts);
+    const at::Tensor qd = dense_last(q, "q");
+    return store(layer, &qd, k, v, rope, start, start_i, counts);
   }
 
   std::tuple<at::Tensor, at::Tensor> read(
       int64_t layer, const c10::optional<at::Tensor>& start, int64_t start_i,
       int64_t n, const c10::optional<at::Tensor>& length, int64_t length_i) {
     const FmaKv8Layer c = at_layer(layer);
-    TORCH_CHECK(n >= 0 && n < (1 << 30) && start_i >= 0 &&
+    TORCH_CHECK_VALUE(n >= 0 && n < (1 << 30) && start_i >= 0 &&
                     start_i < (1 << 30) && length_i >= 0 &&
                     length_i <= c.max_seq,
                 "range outside the cache");
@@ -222,13 +234,14 @@ class Kv8Buffers {
     return {ko, vo};
   }
 
-  at::Tensor attention(const at::Tensor& q, int64_t layer,
+  at::Tensor attention(const at::Tensor& q_in, int64_t layer,
                        const c10::optional<at::Tensor>& start, int64_t start_i,
                        const c10::optional<at::Tensor>& counts, double scale) {
     const FmaKv8Layer c = at_layer(layer);
-    const FmaRows qr = rows_of(q, "q");
+    const at::Tensor q = dense_last(q_in, "q");
+    const FmaRows qr = rows_of(q);
     check_new(q, "q");
-    TORCH_CHECK(q.size(2) >= 1 && q.size(2) % c.kv_heads == 0 &&
+    TORCH_CHECK_VALUE(q.size(2) >= 1 && q.size(2) % c.kv_heads == 0 &&
                     q.size(2) < (1 << 20),
                 "query heads must be a multiple of the cache's kv heads");
     const FmaKv8Span span = span_of(q.size(1), start, start_i, counts);
@@ -256,7 +269,7 @@ class Kv8Buffers {
 
  private:
   FmaKv8Layer at_layer(int64_t layer) const {
-    TORCH_CHECK(layer >= 0 && layer < layers_, "no layer ", layer);
+    TORCH_CHECK_VALUE(layer >= 0 && layer < layers_, "no layer ", layer);
     FmaKv8Layer c = c_;
     c.codes = codes_.data_ptr<uint8_t>() + layer * 2 * c.codes_v;
     c.scales = scales_.data_ptr<float>() + layer * 2 * c.scales_v;
@@ -267,7 +280,7 @@ class Kv8Buffers {
   const int* per_sequence(const c10::optional<at::Tensor>& t,
                           const char* name) const {
     if (!t.has_value()) return nullptr;
-    TORCH_CHECK(t->device() == codes_.device() &&
+    TORCH_CHECK_VALUE(t->device() == codes_.device() &&
                     t->scalar_type() == at::kInt && t->dim() == 1 &&
                     t->size(0) == c_.batch && t->is_contiguous(),
                 name, " must be contiguous int32 [B] beside the cache");
@@ -275,7 +288,7 @@ class Kv8Buffers {
   }
 
   void check_new(const at::Tensor& x, const char* name) const {
-    TORCH_CHECK(x.device() == codes_.device() &&
+    TORCH_CHECK_VALUE(x.device() == codes_.device() &&
                     x.scalar_type() == tail_.scalar_type() &&
                     x.size(0) == c_.batch && x.size(3) == c_.hd &&
                     x.size(1) < (1 << 30),
@@ -291,22 +304,23 @@ class Kv8Buffers {
     s.counts = per_sequence(counts, "counts");
     s.T = static_cast<int>(T);
     if (s.start == nullptr) {
-      TORCH_CHECK(start_i >= 0 && start_i + T <= c_.max_seq,
+      TORCH_CHECK_VALUE(start_i >= 0 && start_i + T <= c_.max_seq,
                   "tokens beyond the cache");
       s.start_i = static_cast<int>(start_i);
     }
     return s;
   }
 
-  at::Tensor store(int64_t layer, const at::Tensor* q, const at::Tensor& k,
-                   const at::Tensor& v, const FmaRope& rope,
+  at::Tensor store(int64_t layer, const at::Tensor* q, const at::Tensor& k_in,
+                   const at::Tensor& v_in, const FmaRope& rope,
                    const c10::optional<at::Tensor>& start, int64_t start_i,
                    const c10::optional<at::Tensor>& counts) {
     const FmaKv8Layer c = at_layer(layer);
-    const FmaRows kr = rows_of(k, "k"), vr = rows_of(v, "v");
+    const at::Tensor k = dense_last(k_in, "k"), v = dense_last(v_in, "v");
+    const FmaRows kr = rows_of(k), vr = rows_of(v);
     check_new(k, "k");
     check_new(v, "v");
-    TORCH_CHECK(k.size(2) == c.kv_heads && v.sizes() == k.sizes(),
+    TORCH_CHECK_VALUE(k.size(2) == c.kv_heads && v.sizes() == k.sizes(),
                 "k and v must be [B, T, kvH, head_dim] of the cache");
     const FmaKv8Span span = span_of(k.size(1), start, start_i, counts);
     FmaRows qr{};
@@ -314,11 +328,11 @@ class Kv8Buffers {
     c10::hip::HIPGuard guard(codes_.device().index());
     int q_heads = 0;
     if (q != nullptr) {
-      qr = rows_of(*q, "q");
+      qr = rows_of(*q);
       check_new(*q, "q");
-      TORCH_CHECK(q->size(1) == k.size(1) && q->size(2) >= 1 &&
-                      q->size(2) < (1 << 20),
-                  "q must be [B, T, qH, head_dim]");
+      TORCH_CHECK_VALUE(q->size(1) == k.size(1) && q->size(2) >= 1 &&
+                      q->size(2) % c.kv_heads == 0 && q->size(2) < (1 << 20),
+                  "q must be [B, T, a multiple of kvH, head_dim]");
       q_heads = static_cast<int>(q->size(2));
       out = at::empty(q->sizes(), tail_.options());
     }

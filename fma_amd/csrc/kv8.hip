@@ -261,6 +261,17 @@ __device__ inline void turn_heads(const Turn<LPR, PAIRS>& turn,
   }
 }
 
+// Which token and which of its items a row of lanes takes: the rows of one
+// wave have the same item of neighbouring tokens, so they end together.
+template <int LPR>
+__device__ inline long long token_of(long long unit, int items, int* item) {
+  constexpr int SIDE = 64 / LPR;
+  const long long rest = unit / SIDE;
+  const long long group = rest / items;
+  *item = static_cast<int>(rest - group * items);
+  return group * SIDE + unit % SIDE;
+}
+
 // A row of LPR lanes takes `per` heads of one token.
 template <typename E, int LPR, bool PAIRS, bool PAST>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(
@@ -271,9 +282,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(
   const long long unit =
       static_cast<long long>(blockIdx.x) * (256 / LPR) + threadIdx.x / LPR;
   const int d0 = (threadIdx.x % LPR) * 8;
-  const long long bt = unit / items;
+  int item;
+  const long long bt = token_of<LPR>(unit, items, &item);
   if (bt >= static_cast<long long>(B) * T) return;
-  const int item = static_cast<int>(unit - bt * items);
   const int b = static_cast<int>(bt / T), t = static_cast<int>(bt - 1LL * b * T);
   const bool is_q = item < q_items;
   const int heads = is_q ? q_heads : kv_heads;
@@ -382,7 +393,9 @@ __device__ inline void scale_of(float amax, float* scale, float* mul) {
 }
 
 template <typename E, int LPR, bool PAIRS, bool FP8, bool PAST>
-__global__ __launch_bounds__(256) void kv8_append_kernel(
+__global__ __launch_bounds__(256, LPR == 32 ? 2
+                                            : PAIRS ? 4
+                                                    : 3) void kv8_append_kernel(
     FmaKv8Layer c, FmaKv8Span sp, FmaRows q, FmaRows k, FmaRows v, void* qo,
     int q_heads, FmaRope r, int blocks, int kv_groups, int per, int q_items) {
   constexpr int MAXD = LPR * 8;
@@ -396,13 +409,17 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(
   float* const my_scratch = scratch + row * LPR * 8;
   const int hd = c.hd;
 
-  if (static_cast<int>(blockIdx.x) >= kv_groups) {
+  // the workgroups of blocks lie among those of queries, so that both run
+  // side by side: block n of kv_groups has number n * stride
+  const int idx = blockIdx.x;
+  const int stride = gridDim.x / kv_groups;
+  if (idx % stride != 0 || idx / stride >= kv_groups) {
     // queries
-    const long long unit =
-        static_cast<long long>(blockIdx.x - kv_groups) * ROWS + row;
-    const long long bt = unit / q_items;
+    int item;
+    const long long bt = token_of<LPR>(
+        static_cast<long long>(idx - min(idx / stride + 1, kv_groups)) * ROWS +
+            row, q_items, &item);
     if (bt >= static_cast<long long>(c.batch) * sp.T) return;
-    const int item = static_cast<int>(unit - bt * q_items);
     const int b = static_cast<int>(bt / sp.T);
     const int t = static_cast<int>(bt - 1LL * b * sp.T);
     const Span s = span_of(sp, b, c.max_seq);
@@ -418,8 +435,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(
   }
 
   // the heads of a block next to each other: their rows are
-  const int h = blockIdx.x % c.kv_heads;
-  const int bj = blockIdx.x / c.kv_heads;
+  const int h = idx / stride % c.kv_heads;
+  const int bj = idx / stride / c.kv_heads;
   const int b = bj / blocks, j = bj - b * blocks;
   const int bh = b * c.kv_heads + h;
   const Span s = span_of(sp, b, c.max_seq);
@@ -495,20 +512,29 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(
   fetch(blk, lo, hi);
   const bool complete = hi == (blk + 1) * BLK;
   if (complete && lo > blk * BLK) {
-    // the block's earlier tokens
+    // the block's earlier tokens, eight values that lie together at a time:
+    // of one token, or of eight
+    const int old = lo - blk * BLK;
     const uint16_t* const kt = tail_at(0, blk);
     const uint16_t* const vt = tail_at(1, blk);
-    for (int i = row; i < lo - blk * BLK; i += ROWS) {
-      if (d0 < c.hdp) {
-        const u16x8 x = *reinterpret_cast<const u16x8*>(kt + kidx(i, d0));
-        u16x8 y;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = vt[vidx(i, d0 + e)];
+    for (int u = tid; u < c.hdp * 4; u += 256) {
+      const u16x8 x = *reinterpret_cast<const u16x8*>(kt + u * 8);
+      u16x8 y = *reinterpret_cast<const u16x8*>(vt + u * 8);
+      const int e = u & 1, l = (u >> 1) & 63, chunk = u >> 7;
+      const int g = l >> 4, n = l & 15;
+      if (16 * e + n < old) {
         note(0, x);
-        note(1, y);
-        *reinterpret_cast<u16x8*>(&tile[0][i][d0]) = x;
-        *reinterpret_cast<u16x8*>(&tile[1][i][d0]) = y;
+        *reinterpret_cast<u16x8*>(&tile[0][16 * e + n][32 * chunk + 8 * g]) = x;
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int tok = 16 * (i >> 2) + 4 * g + (i & 3);
+        if (tok < old)
+          tile[1][tok][32 * chunk + 16 * e + n] = y[i];
+        else
+          y[i] = 0;
+      }
+      note(1, y);
     }
   }
   if (complete) {
@@ -945,8 +971,9 @@ __device__ inline float query_fp16(const AttnArgs& A, const u16x8 (&raw)[NS],
 }
 
 // The incomplete block, raw, for 16 rows. Its weights go in as two 16-bit
-// parts: a single bf16 would cost as much as the result's rounding.
-template <int NS, typename E>
+// parts: a single bf16 would cost as much as the result's rounding. HOLD: V
+// stays in registers, else it is read twice.
+template <int NS, typename E, bool HOLD>
 __device__ inline void tail_step(const AttnArgs& A, const Reach& R, int bh,
                                  int lane, const u16x8 (&q)[NS], int seen,
                                  RowState<NS> (&state)[1]) {
@@ -957,6 +984,17 @@ __device__ inline void tail_step(const AttnArgs& A, const Reach& R, int bh,
       (static_cast<long long>(bh) * 2 + (R.full & 1)) * BLK * NS * 32 +
       lane * 16;
   const uint16_t* const vt = kt + A.c.tail_v;
+  u16x8 v[HOLD ? 2 * NS : 1];
+  u16x8 most = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+  for (int n = 0; n < 2 * NS; ++n) {
+    u16x8& y = v[HOLD ? n : 0];
+    y = *reinterpret_cast<const u16x8*>(vt + (n >> 1) * 1024 + (n & 1) * 8);
+    most = __builtin_elementwise_max(most, y & static_cast<uint16_t>(0x7fff));
+  }
+  uint32_t wild = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) wild = max(wild, static_cast<uint32_t>(most[i]));
   f32x4 xs[1][1][2] = {{{{0, 0, 0, 0}, {0, 0, 0, 0}}}};
   f32x4(&x)[2] = xs[0][0];
 #pragma unroll
@@ -982,23 +1020,37 @@ __device__ inline void tail_step(const AttnArgs& A, const Reach& R, int bh,
       hi[4 * a + r] = u;
       lo[4 * a + r] = E::from_f(x[a][r] - E::to_f(u));
     }
+  // NaN or infinities, in tokens or behind them
+  const bool tamed = __any(wild >= E::kInf);
   const int held = R.s.end - R.full * BLK - 4 * g;
 #pragma unroll
   for (int n = 0; n < 2 * NS; ++n) {
-    u16x8 v = *reinterpret_cast<const u16x8*>(vt + (n >> 1) * 1024 +
-                                              (n & 1) * 8);
+    u16x8& y = v[HOLD ? n : 0];
+    if (!HOLD)
+      y = *reinterpret_cast<const u16x8*>(vt + (n >> 1) * 1024 + (n & 1) * 8);
+    if (tamed) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v[i] = 16 * (i >> 2) + (i & 3) < held ? tame<E>(v[i]) : 0;
-    st.o[n] = mfma16<E>(v, hi, st.o[n]);
-    st.o[n] = mfma16<E>(v, lo, st.o[n]);
+      for (int i = 0; i < 8; ++i)
+        y[i] = 16 * (i >> 2) + (i & 3) < held ? tame<E>(y[i]) : 0;
+    }
+    st.o[n] = mfma16<E>(y, hi, st.o[n]);
+    st.o[n] = mfma16<E>(y, lo, st.o[n]);
   }
 }
 
 // Few rows: four waves share 16 rows and take the blocks of a split in turn,
 // each straight from memory into the matrix unit's operands, the next block
 // on its way meanwhile.
-template <int NS, bool FP8, typename E>
+// PAST: codes that no cache would keep until they are read again are not put
+// there (270 MB: 58 us against 67 us).
+template <bool PAST, typename V>
+__device__ inline V get(const void* at) {
+  if constexpr (PAST)
+    return __builtin_nontemporal_load(static_cast<const V*>(at));
+  else
+    return *static_cast<const V*>(at);
+}
+template <int NS, bool FP8, typename E, bool PAST>
 __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(AttnArgs A) {
   constexpr int HDP = NS * 32;
   __shared__ float s_o[4][16][HDP + 4];
@@ -1023,13 +1075,6 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
   st.clear();
 
   if (R.lo < R.hi || R.tail) {
-    const uint16_t* const qrow = static_cast<const uint16_t*>(A.q.p) +
-                                 b * A.q.sb + t * A.q.st + hq * A.q.sh;
-    u16x8 raw[NS];
-    h8 q[NS];
-    load_query<NS, E>(A, qrow, live, g, raw);
-    const float qscale = query_fp16<NS, E>(A, raw, q);
-
     const unsigned char* const kc =
         c.codes + static_cast<long long>(bh) * c.nblk * BLK * HDP + lane * 16;
     const unsigned char* const vc = kc + c.codes_v;
@@ -1039,21 +1084,35 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
     ScaleRef<FP8> vs;
     u32x4 kr[NS], vr[NS];
     float k_next = 0.0f, v_next = 0.0f;
-    auto load = [&](int blk) {
+    // wide heads have no registers for the next V beside this one's
+    constexpr bool AHEAD = NS <= 4;
+    auto load_k = [&](int blk) {
       const long long at = static_cast<long long>(blk) * BLK * HDP;
 #pragma unroll
       for (int i = 0; i < NS; ++i)
-        kr[i] = *reinterpret_cast<const u32x4*>(kc + at + i * 1024);
+        kr[i] = get<PAST, u32x4>(kc + at + i * 1024);
+      k_next = ksc[blk];
+    };
+    auto load_v = [&](int blk) {
+      const long long at = static_cast<long long>(blk) * BLK * HDP;
 #pragma unroll
       for (int i = 0; i < NS; ++i)
-        vr[i] = *reinterpret_cast<const u32x4*>(vc + at + i * 1024);
-      k_next = ksc[blk];
+        vr[i] = get<PAST, u32x4>(vc + at + i * 1024);
       v_next = vsc[blk];
     };
     int blk = R.lo + wave;
-    if (blk < R.hi) load(blk);
+    if (blk < R.hi) {
+      load_k(blk);
+      load_v(blk);
+    }
+    const uint16_t* const qrow = static_cast<const uint16_t*>(A.q.p) +
+                                 b * A.q.sb + t * A.q.st + hq * A.q.sh;
+    u16x8 raw[NS];
+    h8 q[NS];
+    load_query<NS, E>(A, qrow, live, g, raw);
+    const float qscale = query_fp16<NS, E>(A, raw, q);
     for (; blk < R.hi; blk += 4) {
-      const float kscale = k_next, vscale = v_next;
+      const float kscale = k_next;
       f32x4 xs[1][1][2] = {{{{0, 0, 0, 0}, {0, 0, 0, 0}}}};
       f32x4(&x)[2] = xs[0][0];
 #pragma unroll
@@ -1063,10 +1122,14 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
         x[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
             decode8(kr[ks][2], kr[ks][3], 1.0f, FP8), q[ks], x[1], 0, 0, 0);
       }
+      const float vscale = v_next;
       u32x4 v_now[NS];
 #pragma unroll
       for (int i = 0; i < NS; ++i) v_now[i] = vr[i];
-      if (blk + 4 < R.hi) load(blk + 4);
+      if (blk + 4 < R.hi) {
+        load_k(blk + 4);
+        if (AHEAD) load_v(blk + 4);
+      }
       const float f[1][1] = {{factor(kscale, qscale)}};
       mask(x, seen - blk * BLK - 4 * g);
       settle<NS, 1, 1>(xs, f, state, vs.follow(vscale));
@@ -1082,11 +1145,12 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
             decode8(v_now[i][2], v_now[i][3], ratio, FP8), p, st.o[2 * i + 1],
             0, 0, 0);
       }
+      if (!AHEAD && blk + 4 < R.hi) load_v(blk + 4);
     }
     st.times(vs.ref);
     if (R.tail && wave == 3) {
       load_query<NS, E>(A, qrow, live, g, raw);
-      tail_step<NS, E>(A, R, bh, lane, raw, seen, state);
+      tail_step<NS, E, (NS <= 4)>(A, R, bh, lane, raw, seen, state);
     }
   }
 
@@ -1310,7 +1374,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
     for (int r = 0; r < NR; ++r) {
       u16x8 raw[NS];
       load_query<NS, E>(A, qrow[r], live[r], g, raw);
-      tail_step<NS, E>(A, R, bh, lane, raw, seen[r],
+      tail_step<NS, E, false>(A, R, bh, lane, raw, seen[r],
                        *reinterpret_cast<RowState<NS>(*)[1]>(&st[r]));
     }
   }
@@ -1423,15 +1487,24 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(const float* partials,
 // Heads that a row of lanes takes: as many as leave every CU six workgroups
 // of 256 threads, at most 16 (8192 tokens of 32 + 8 heads: 4 heads 38.6 us, 8
 // 34.7 us, 16 31.7 us, 32 37.9 us).
-int heads_each(long long rows) {
+int heads_each(long long rows, int heads) {
   const long long n = rows / (256 * 6 * 16);
-  return n < 1 ? 1 : n > 16 ? 16 : static_cast<int>(n);
+  const int most = n < 1 ? 1 : n > 16 ? 16 : static_cast<int>(n);
+  const int items = (heads + most - 1) / most;  // of like size
+  return (heads + items - 1) / items;
 }
 // Outputs beyond the 32 MB of second-level caches are stored past them: at
 // 84 MB 37.8 us against 50.7 us.
 bool past_caches(long long bytes) { return bytes > (32LL << 20); }
 
 int lanes_per_row(int hd) { return hd <= 64 ? 8 : hd <= 128 ? 16 : 32; }
+
+// Workgroups for `items` rows of lanes a token, as token_of hands them out.
+long long token_groups(long long tokens, int items, int hd) {
+  const int rows = 256 / lanes_per_row(hd), side = 64 / lanes_per_row(hd);
+  const long long units = (tokens + side - 1) / side * side * items;
+  return (units + rows - 1) / rows;
+}
 
 template <typename... P, typename... Given>
 hipError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t lds,
@@ -1476,11 +1549,10 @@ extern "C" hipError_t fma_launch_qk_norm_rope(
     hipStream_t stream) {
   const long long tokens = static_cast<long long>(B) * T;
   if (tokens == 0) return hipSuccess;
-  const int per = heads_each(tokens * (q_heads + kv_heads));
+  const int per = heads_each(tokens * (q_heads + kv_heads), q_heads);
   const int q_items = (q_heads + per - 1) / per;
   const int items = q_items + (kv_heads + per - 1) / per;
-  const int rows = 256 / lanes_per_row(hd);
-  const long long grid = (tokens * items + rows - 1) / rows;
+  const long long grid = token_groups(tokens, items, hd);
   if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
   FMA_BY_TYPE(type, FMA_BY_LANES(hd, FMA_BY_BOOL(rope.pairs, PAIRS,
       FMA_BY_BOOL(past_caches(tokens * (q_heads + kv_heads) * hd *
@@ -1502,11 +1574,10 @@ extern "C" hipError_t fma_launch_kv8_append(FmaKv8Layer c, FmaKv8Span span,
     blocks = (span.start_i + span.T - 1) / BLK - span.start_i / BLK + 1;
   const long long kv_groups =
       static_cast<long long>(c.batch) * c.kv_heads * blocks;
-  const int per = heads_each(tokens * q_heads);
+  const int per = heads_each(tokens * q_heads, q_heads > 0 ? q_heads : 1);
   const int q_items = (q_heads + per - 1) / per;
-  const int rows = 256 / lanes_per_row(c.hd);
   const long long q_groups =
-      q.p == nullptr ? 0 : (tokens * q_items + rows - 1) / rows;
+      q.p == nullptr ? 0 : token_groups(tokens, q_items, c.hd);
   if (kv_groups + q_groups > 0x7fffffffLL) return hipErrorInvalidValue;
   const unsigned grid = static_cast<unsigned>(kv_groups + q_groups);
   FMA_BY_TYPE16(c.bf16, FMA_BY_LANES(c.hd, FMA_BY_BOOL(rope.pairs, PAIRS,
@@ -1552,8 +1623,11 @@ extern "C" int fma_kv8_attn_splits(const FmaKv8Layer* c, int T, int q_heads,
   const long long groups =
       (rows + tile - 1) / tile * c->batch * c->kv_heads;
   const int nb = max_len / BLK;
-  // two workgroups a CU, and at least a block for each wave
-  long long splits = groups > 0 ? 2LL * cus / groups : 1;
+  // Four workgroups a CU (two of many rows), for sequences of different
+  // length to even out, and at least a block for each wave: 32 sequences of
+  // up to 8192 tokens, 8 kv heads, 1 / 2 / 4 / 8 / 16 splits took
+  // 74.0 / 61.5 / 58.1 / 60.0 / 66.4 us.
+  long long splits = groups > 0 ? (tile == 16 ? 4LL : 2LL) * cus / groups : 1;
   if (splits > nb / 4) splits = nb / 4;
   return splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : static_cast<int>(splits);
 }
@@ -1586,11 +1660,16 @@ extern "C" hipError_t fma_launch_kv8_attention(FmaKv8Layer c, FmaKv8Span span,
   a.rows = static_cast<int>(rows);
   a.tiles = static_cast<int>(tiles);
   a.splits = splits;
+  const long long held =
+      span.start == nullptr ? span.start_i + span.T : c.max_seq;
+  const bool past = past_caches(2 * held * c.batch * c.kv_heads * c.hdp);
   hipError_t err = hipSuccess;
   const dim3 g(static_cast<unsigned>(grid));
   if (tile == 16) {
     FMA_BY_TYPE16(c.bf16, FMA_BY_BOOL(c.fp8, FP8, FMA_BY_WIDTH(c.hdp,
-        err = launch(kv8_attn_few_kernel<NS, FP8, E>, g, 256, 0, stream, a))));
+        FMA_BY_BOOL(past, PAST,
+            err = launch(kv8_attn_few_kernel<NS, FP8, E, PAST>, g, 256, 0,
+                         stream, a)))));
   } else {
     FMA_BY_TYPE16(c.bf16, FMA_BY_BOOL(c.fp8, FP8, FMA_BY_WIDTH(c.hdp,
         err = launch(kv8_attn_many_kernel<NS, FP8, E, many_nr(NS), many_ne(NS)>,

@@ -119,6 +119,11 @@ def fast_qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor,
     it; one that only the GPU knows gives NaN.
 
     One launch on the GPU for any T; torch operations on the CPU."""
+    if q.is_cuda:
+        given = isinstance(pos, torch.Tensor)
+        return actuation.require_native().qk_norm_rope(
+            q, k, cos, sin, pos if given else None, 0 if given else pos,
+            q_norm, k_norm, eps, interleaved)
     if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] \
             or q.shape[3] != k.shape[3] or q.shape[2] < 1 or k.shape[2] < 1:
         raise ValueError(f"q {list(q.shape)} and k {list(k.shape)} must be "
@@ -144,14 +149,6 @@ def fast_qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor,
     elif pos < 0 or pos + T > cos.shape[0]:
         raise ValueError(f"positions [{pos}, {pos + T}) lie outside the "
                          f"tables' {cos.shape[0]}")
-    if q.stride(3) != 1:
-        q = q.contiguous()
-    if k.stride(3) != 1:
-        k = k.contiguous()
-    if q.is_cuda:
-        return actuation.require_native().qk_norm_rope(
-            q, k, cos, sin, pos if given else None, 0 if given else pos,
-            q_norm, k_norm, float(eps), interleaved)
     if not given:
         pos = torch.full((B,), pos, dtype=torch.long)
     if pos.dim() == 1:

@@ -121,52 +121,57 @@ class KV8Cache:
             raise ValueError(f"{name} requires a gradient; the 8-bit cache "
                              "has no backward pass")
 
+    def _check_span(self, *given: Optional[Position]) -> None:
+        for t in given:
+            if isinstance(t, torch.Tensor):
+                self._check_ints(t, "start, counts or length")
+
     def _check_ints(self, t: torch.Tensor, name: str) -> None:
         if t.dtype != torch.int32 or t.shape != (self.batch,) \
                 or t.device != self.device or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous int32 "
                              f"[{self.batch}] on {self.device}")
 
-    def _span(self, layer: int, start: Position, T: int,
-              counts: Optional[torch.Tensor], store: bool
-              ) -> Tuple[Optional[torch.Tensor], int]:
-        if counts is not None:
-            self._check_ints(counts, "counts")
-        known = self._length[layer]
-        if isinstance(start, torch.Tensor):
-            self._check_ints(start, "start")
-            if store and T:
-                self._length[layer] = None
-            return start, 0
+    def _may(self, layer: int, start: int, T: int, store: bool,
+             counts: Optional[torch.Tensor]) -> None:
+        """Refuse what does not fit the tokens held, as far as the host knows
+        them."""
         end = start + T
         if start < 0 or end > self.max_seq:
             raise ValueError(f"tokens [{start}, {end}) lie outside the "
                              f"cache's {self.max_seq}")
+        known = self._length[layer]
+        if known is None or not T:
+            return
         if not store:
-            if known is not None and counts is None and end > known:
+            if counts is None and end > known:
                 raise ValueError(f"attention over {end} tokens, but the "
                                  f"cache holds {known}")
-            return None, start
-        if known is None and start == 0 and counts is None and T:
-            self._length[layer] = end
-            self._raw_from[layer] = max((end // BLOCK - 1) * BLOCK, 0)
-        elif known is not None and T:
-            if start > known:
-                raise ValueError(f"appending at {start} would leave a hole "
-                                 f"behind the {known} tokens held")
-            raw = self._raw_from[layer]
-            if start % BLOCK and start < raw:
-                raise ValueError(
-                    f"cannot append at {start}: raw values are held from "
-                    f"{raw} on (or start at a multiple of {BLOCK})")
-            if counts is not None:
-                self._length[layer] = None
-            else:
-                self._length[layer] = end
-                self._raw_from[layer] = max(
-                    min(raw, start // BLOCK * BLOCK),
-                    (end // BLOCK - 1) * BLOCK, 0)
-        return None, start
+        elif start > known:
+            raise ValueError(f"appending at {start} would leave a hole "
+                             f"behind the {known} tokens held")
+        elif start % BLOCK and start < self._raw_from[layer]:
+            raise ValueError(
+                f"cannot append at {start}: raw values are held from "
+                f"{self._raw_from[layer]} on (or start at a multiple of "
+                f"{BLOCK})")
+
+    def _stored(self, layer: int, start: Position, T: int,
+                counts: Optional[torch.Tensor]) -> None:
+        if not T:
+            return
+        if counts is not None or isinstance(start, torch.Tensor):
+            self._length[layer] = None
+            return
+        known, end = self._length[layer], start + T
+        if known is None:
+            if start:
+                return
+            self._raw_from[layer] = 0
+        self._length[layer] = end
+        self._raw_from[layer] = max(
+            min(self._raw_from[layer], start // BLOCK * BLOCK),
+            (end // BLOCK - 1) * BLOCK)
 
 
 def _check_pair(q: torch.Tensor, k: torch.Tensor) -> None:
@@ -183,15 +188,20 @@ def kv8_append(cache: KV8Cache, layer: int, k: torch.Tensor, v: torch.Tensor,
     how many of the T tokens are each sequence's own, the rest is padding.
     Any strides but a contiguous last dimension."""
     cache._check_layer(layer)
-    cache._check_rows(k, "k", cache.kv_heads)
-    cache._check_rows(v, "v", cache.kv_heads)
-    _check_pair(v, k)
-    k, v = _dense_last(k), _dense_last(v)
-    at, at_i = cache._span(layer, start, k.shape[1], counts, True)
+    given = isinstance(start, torch.Tensor)
+    T = k.shape[1] if k.dim() == 4 else 0
+    if not given:
+        cache._may(layer, start, T, True, counts)
     if cache._native is not None:
-        cache._native.append(layer, k, v, at, at_i, counts)
+        cache._native.append(layer, k, v, start if given else None,
+                             0 if given else start, counts)
     else:
+        cache._check_rows(k, "k", cache.kv_heads)
+        cache._check_rows(v, "v", cache.kv_heads)
+        _check_pair(v, k)
+        cache._check_span(start, counts)
         _store(cache, layer, k, v, start, counts)
+    cache._stored(layer, start, T, counts)
 
 
 def qk_norm_rope_kv8(cache: KV8Cache, layer: int, q: torch.Tensor,
@@ -206,24 +216,28 @@ def qk_norm_rope_kv8(cache: KV8Cache, layer: int, q: torch.Tensor,
     positions start.. and :func:`kv8_append` of the result and v, in one
     launch; the same bits as the two calls. Returns the queries, zeros behind
     each sequence's count. The tables must cover the cache's max_seq."""
-    from fma_amd.ops.decode_ops import (_check_rope, rope_rows)
     cache._check_layer(layer)
+    given = isinstance(start, torch.Tensor)
+    T = k.shape[1] if k.dim() == 4 else 0
+    if not given:
+        cache._may(layer, start, T, True, counts)
+    if cache._native is not None:
+        out = cache._native.norm_rope_append(
+            layer, q, k, v, cos, sin, start if given else None,
+            0 if given else start, q_norm, k_norm, counts, eps, interleaved)
+        cache._stored(layer, start, T, counts)
+        return out
+    from fma_amd.ops.decode_ops import _check_rope, rope_rows
     cache._check_rows(q, "q", 0)
     cache._check_rows(k, "k", cache.kv_heads)
     cache._check_rows(v, "v", cache.kv_heads)
     _check_pair(q, k)
     _check_pair(v, k)
     _check_rope(q, k, cos, sin, q_norm, k_norm)
+    cache._check_span(start, counts)
     if cos.shape[0] < cache.max_seq:
         raise ValueError(f"the cos/sin tables hold {cos.shape[0]} positions, "
                          f"the cache {cache.max_seq}")
-    q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
-    at, at_i = cache._span(layer, start, k.shape[1], counts, True)
-    if cache._native is not None:
-        return cache._native.norm_rope_append(
-            layer, q, k, v, cos, sin, at, at_i, q_norm, k_norm, counts,
-            float(eps), interleaved)
-    B, T = q.shape[:2]
     starts, ns = _host_span(cache, start, T, counts)
     pos = starts[:, None] + torch.arange(T)
     pos = pos.clamp(0, cache.max_seq - 1)
@@ -231,6 +245,7 @@ def qk_norm_rope_kv8(cache: KV8Cache, layer: int, q: torch.Tensor,
     qo = rope_rows(q, q_norm, cos, sin, pos, eps, interleaved)
     ko = rope_rows(k, k_norm, cos, sin, pos, eps, interleaved)
     _store(cache, layer, ko, v, start, counts)
+    cache._stored(layer, start, T, counts)
     return torch.where(live, qo, torch.zeros((), dtype=qo.dtype))
 
 
@@ -243,14 +258,17 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, layer: int,
     multiple of kvH. start and counts as in :func:`kv8_append`; rows behind a
     sequence's count come out as zeros."""
     cache._check_layer(layer)
-    cache._check_rows(q, "q", 0)
-    q = _dense_last(q)
-    at, at_i = cache._span(layer, start, q.shape[1], counts, False)
+    given = isinstance(start, torch.Tensor)
+    if not given:
+        cache._may(layer, start, q.shape[1] if q.dim() == 4 else 0, False,
+                   counts)
     if scale is None:
         scale = cache.head_dim ** -0.5
     if cache._native is not None:
-        return cache._native.attention(q, layer, at, at_i, counts,
-                                       float(scale))
+        return cache._native.attention(q, layer, start if given else None,
+                                       0 if given else start, counts, scale)
+    cache._check_rows(q, "q", 0)
+    cache._check_span(start, counts)
     return _attend(q, cache, layer, start, counts, scale)
 
 
@@ -265,7 +283,6 @@ def kv8_read(cache: KV8Cache, layer: int, start: Position, n: int,
     args = []
     for value, name in ((start, "start"), (length, "length")):
         if isinstance(value, torch.Tensor):
-            cache._check_ints(value, name)
             args += [value, 0]
         else:
             if not 0 <= value <= cache.max_seq:
@@ -275,6 +292,7 @@ def kv8_read(cache: KV8Cache, layer: int, start: Position, n: int,
     if cache._native is not None:
         return cache._native.read(layer, args[0], args[1], n, args[2],
                                   args[3])
+    cache._check_span(args[0], args[2])
     out = torch.zeros((2, cache.batch, n, cache.kv_heads, cache.head_dim),
                       dtype=cache.dtype)
     for b in range(cache.batch):
@@ -286,10 +304,6 @@ def kv8_read(cache: KV8Cache, layer: int, start: Position, n: int,
             for w, x in enumerate(_held(cache, layer, b, end)):
                 out[w, b, :m] = x[s:s + m].to(cache.dtype)
     return out[0], out[1]
-
-
-def _dense_last(x: torch.Tensor) -> torch.Tensor:
-    return x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous()
 
 
 # -- the same on the CPU -------------------------------------------------------
