@@ -26,6 +26,10 @@ int compute_units(int device) {
   return at::cuda::getDeviceProperties(device)->multiProcessorCount;
 }
 
+bool aligned16(const void* p) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0;
+}
+
 // [B, T, H, hd], copied if its last dimension is not contiguous.
 at::Tensor dense_last(const at::Tensor& x, const char* name) {
   TORCH_CHECK_VALUE(x.is_cuda() && x.dim() == 4, name,
@@ -45,7 +49,7 @@ FmaRows rows_of(const at::Tensor& x) {
   auto aligned = [&](int64_t stride, int64_t n) {
     return n <= 1 || (stride * size) % 16 == 0;
   };
-  r.vec = reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && x.size(3) % 8 == 0 &&
+  r.vec = aligned16(r.p) && x.size(3) % 8 == 0 &&
           aligned(r.sb, x.size(0)) && aligned(r.st, x.size(1)) &&
           aligned(r.sh, x.size(2));
   return r;
@@ -81,6 +85,7 @@ FmaRope rope_of(const c10::optional<at::Tensor>& cos,
     r.sin = s.data_ptr<float>();
     r.half = static_cast<int>(c.size(1));
     r.table = static_cast<int>(c.size(0));
+    r.tab_vec = r.half % 4 == 0 && aligned16(r.cos) && aligned16(r.sin);
   }
   auto weight = [&](const c10::optional<at::Tensor>& w) -> const void* {
     if (!w.has_value()) return nullptr;
@@ -92,6 +97,7 @@ FmaRope rope_of(const c10::optional<at::Tensor>& cos,
   };
   r.qw = weight(qw);
   r.kw = weight(kw);
+  r.w_vec = hd % 8 == 0 && aligned16(r.qw) && aligned16(r.kw);
   return r;
 }
 

@@ -52,6 +52,8 @@ struct FmaRope {
   float eps;
   const void* qw;
   const void* kw;
+  int tab_vec;   // rows of the tables start on 16-byte borders
+  int w_vec;     // the gains too, and hd % 8 == 0
 };
 
 // position of token (b, t): base + b * sb + t * st of an int32 / int64
