@@ -244,15 +244,23 @@ class Kv8Buffers {
                        const c10::optional<at::Tensor>& start, int64_t start_i,
                        const c10::optional<at::Tensor>& counts, double scale) {
     const FmaKv8Layer c = at_layer(layer);
-    const at::Tensor q = dense_last(q_in, "q");
-    const FmaRows qr = rows_of(q);
+    at::Tensor q = dense_last(q_in, "q");
     check_new(q, "q");
+    FmaRows qr = rows_of(q);
+    if (!qr.vec) {
+      // the kernel takes rows by 16 bytes
+      q = at::constant_pad_nd(q, {0, (8 - c.hd % 8) % 8}).contiguous();
+      if (!aligned16(q.data_ptr()) || q.data_ptr() == q_in.data_ptr())
+        q = q.clone(at::MemoryFormat::Contiguous);
+      qr = rows_of(q);
+      TORCH_CHECK(qr.vec, "rows of q are not aligned");
+    }
     TORCH_CHECK_VALUE(q.size(2) >= 1 && q.size(2) % c.kv_heads == 0 &&
                     q.size(2) < (1 << 20),
                 "query heads must be a multiple of the cache's kv heads");
     const FmaKv8Span span = span_of(q.size(1), start, start_i, counts);
     c10::hip::HIPGuard guard(q.device().index());
-    auto out = at::empty(q.sizes(), tail_.options());
+    auto out = at::empty(q_in.sizes(), tail_.options());
     auto stream = c10::hip::getCurrentHIPStream(q.device().index());
     const int q_heads = static_cast<int>(q.size(2));
     const int max_len = span.start != nullptr

@@ -1026,15 +1026,8 @@ __device__ inline void load_query(const AttnArgs& A, const uint16_t* row,
   for (int ks = 0; ks < NS; ++ks) {
     const int d = 32 * ks + 8 * g;
     raw[ks] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
-    if (live && d < A.c.hd) {
-      if (A.q.vec) {
-        raw[ks] = *reinterpret_cast<const u16x8*>(row + d);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (d + i < A.c.hd) raw[ks][i] = row[d + i];
-      }
-    }
+    if (live && d < A.c.hd)  // rows are padded to 16 bytes
+      raw[ks] = *reinterpret_cast<const u16x8*>(row + d);
   }
 }
 // Returns what makes products of codes log2 scores, but for K's scale.
@@ -1060,71 +1053,94 @@ __device__ inline float query_fp16(const AttnArgs& A, const u16x8 (&raw)[NS],
   return A.scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 }
 
-// The incomplete block, raw, for 16 rows. Its weights go in as two 16-bit
-// parts: a single bf16 would cost as much as the result's rounding. HOLD: V
-// stays in registers, else it is read twice.
-template <int NS, typename E, bool HOLD>
+// The incomplete block, raw, for NR times 16 rows. Its weights go in as two
+// 16-bit parts: a single bf16 would cost as much as the result's rounding.
+template <int NS, int NR, typename E>
 __device__ inline void tail_step(const AttnArgs& A, const Reach& R, int bh,
-                                 int lane, const u16x8 (&q)[NS], int seen,
-                                 RowState<NS> (&state)[1]) {
-  RowState<NS>& st = state[0];
+                                 int lane, const u16x8 (&q)[NR][NS],
+                                 const int (&seen)[NR],
+                                 RowState<NS> (&st)[NR]) {
   const int g = lane >> 4;
   const uint16_t* const kt =
       static_cast<const uint16_t*>(A.c.tail) +
       (static_cast<long long>(bh) * 2 + (R.full & 1)) * BLK * NS * 32 +
       lane * 16;
   const uint16_t* const vt = kt + A.c.tail_v;
-  u16x8 v[HOLD ? 2 * NS : 1];
-  u16x8 most = {0, 0, 0, 0, 0, 0, 0, 0};
+  f32x4 x[1][NR][2];
+  float f[1][NR];
 #pragma unroll
-  for (int n = 0; n < 2 * NS; ++n) {
-    u16x8& y = v[HOLD ? n : 0];
-    y = *reinterpret_cast<const u16x8*>(vt + (n >> 1) * 1024 + (n & 1) * 8);
-    most = __builtin_elementwise_max(most, y & static_cast<uint16_t>(0x7fff));
+  for (int r = 0; r < NR; ++r) {
+    x[0][r][0] = x[0][r][1] = f32x4{0, 0, 0, 0};
+    f[0][r] = A.scale;
   }
-  uint32_t wild = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) wild = max(wild, static_cast<uint32_t>(most[i]));
-  f32x4 xs[1][1][2] = {{{{0, 0, 0, 0}, {0, 0, 0, 0}}}};
-  f32x4(&x)[2] = xs[0][0];
 #pragma unroll
   for (int ks = 0; ks < NS; ++ks)
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
-      x[a] = mfma16<E>(*reinterpret_cast<const u16x8*>(kt + ks * 1024 + a * 8),
-                       q[ks], x[a]);
-  if (A.negative) {
-    x[0] = -x[0];
-    x[1] = -x[1];
-  }
-  mask(x, seen - R.full * BLK - 4 * g);
-  const float f[1][1] = {{A.scale}};
-  settle<NS, 1, 1>(xs, f, state, 1.0f);
-  weigh<NS>(x, A.scale, st);
-  u16x8 hi, lo;
+    for (int a = 0; a < 2; ++a) {
+      const u16x8 k = *reinterpret_cast<const u16x8*>(kt + ks * 1024 + a * 8);
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const uint16_t u = E::from_f(x[a][r]);
-      hi[4 * a + r] = u;
-      lo[4 * a + r] = E::from_f(x[a][r] - E::to_f(u));
+      for (int r = 0; r < NR; ++r)
+        x[0][r][a] = mfma16<E>(k, q[r][ks], x[0][r][a]);
     }
-  // NaN or infinities, in tokens or behind them
-  const bool tamed = __any(wild >= E::kInf);
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    if (A.negative) {
+      x[0][r][0] = -x[0][r][0];
+      x[0][r][1] = -x[0][r][1];
+    }
+    mask(x[0][r], seen[r] - R.full * BLK - 4 * g);
+  }
+  settle<NS, NR, 1>(x, f, st, 1.0f);
+  u16x8 hi[NR], lo[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    weigh<NS>(x[0][r], A.scale, st[r]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float p = x[0][r][i >> 2][i & 3];
+      const uint16_t u = E::from_f(p);
+      hi[r][i] = u;
+      lo[r][i] = E::from_f(p - E::to_f(u));
+    }
+  }
   const int held = R.s.end - R.full * BLK - 4 * g;
 #pragma unroll
   for (int n = 0; n < 2 * NS; ++n) {
-    u16x8& y = v[HOLD ? n : 0];
-    if (!HOLD)
-      y = *reinterpret_cast<const u16x8*>(vt + (n >> 1) * 1024 + (n & 1) * 8);
-    if (tamed) {
+    u16x8 v = *reinterpret_cast<const u16x8*>(vt + (n >> 1) * 1024 +
+                                              (n & 1) * 8);
+    const u16x8 m = v & static_cast<uint16_t>(0x7fff);
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, static_cast<uint32_t>(m[i]));
+    if (__builtin_expect(__any(most >= E::kInf), 0)) {
+      // NaN or infinities, in tokens or behind them
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        y[i] = 16 * (i >> 2) + (i & 3) < held ? tame<E>(y[i]) : 0;
+        v[i] = 16 * (i >> 2) + (i & 3) < held ? tame<E>(v[i]) : 0;
     }
-    st.o[n] = mfma16<E>(y, hi, st.o[n]);
-    st.o[n] = mfma16<E>(y, lo, st.o[n]);
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      st[r].o[n] = mfma16<E>(v, hi[r], st[r].o[n]);
+      st[r].o[n] = mfma16<E>(v, lo[r], st[r].o[n]);
+    }
+  }
+}
+
+// Four values of an output row, o / sum; nothing seen gives zeros.
+template <typename E>
+__device__ inline void put_row(uint16_t* row, int d, int hd, f32x4 o,
+                               float sum) {
+  const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+  typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+  u16x4 u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u[i] = E::from_f(o[i] * by);
+  if (hd % 4 == 0) {
+    if (d < hd) *reinterpret_cast<u16x4*>(row + d) = u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d + i < hd) row[d + i] = u[i];
   }
 }
 
@@ -1197,10 +1213,10 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
     }
     const uint16_t* const qrow = static_cast<const uint16_t*>(A.q.p) +
                                  b * A.q.sb + t * A.q.st + hq * A.q.sh;
-    u16x8 raw[NS];
+    u16x8 raw[1][NS];
     h8 q[NS];
-    load_query<NS, E>(A, qrow, live, g, raw);
-    const float qscale = query_fp16<NS, E>(A, raw, q);
+    load_query<NS, E>(A, qrow, live, g, raw[0]);
+    const float qscale = query_fp16<NS, E>(A, raw[0], q);
     for (; blk < R.hi; blk += 4) {
       const float kscale = k_next;
       f32x4 xs[1][1][2] = {{{{0, 0, 0, 0}, {0, 0, 0, 0}}}};
@@ -1239,8 +1255,9 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
     }
     st.times(vs.ref);
     if (R.tail && wave == 3) {
-      load_query<NS, E>(A, qrow, live, g, raw);
-      tail_step<NS, E, (NS <= 4)>(A, R, bh, lane, raw, seen, state);
+      load_query<NS, E>(A, qrow, live, g, raw[0]);
+      const int sees[1] = {seen};
+      tail_step<NS, 1, E>(A, R, bh, lane, raw, sees, state);
     }
   }
 
@@ -1256,32 +1273,32 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
     s_l[wave][n16] = l;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * HDP; i += 256) {
-    const int rr = i / HDP, d = i - rr * HDP;
+  for (int i = threadIdx.x; i < 4 * HDP; i += 256) {
+    const int rr = i / (HDP / 4), d = i % (HDP / 4) * 4;
     const int orow = tile * 16 + rr;
     if (orow >= A.rows) continue;
     const float m = fmaxf(fmaxf(s_m[0][rr], s_m[1][rr]),
                           fmaxf(s_m[2][rr], s_m[3][rr]));
-    float o = 0.0f, sum = 0.0f;
+    f32x4 o = {0, 0, 0, 0};
+    float sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float f = exp2f(s_m[w][rr] - m);
-      o += s_o[w][rr][d] * f;
+      const float f = __builtin_amdgcn_exp2f(s_m[w][rr] - m);
+      o += *reinterpret_cast<const f32x4*>(&s_o[w][rr][d]) * f;
       sum += s_l[w][rr] * f;
     }
     const int ot = orow / A.group, oh = h * A.group + (orow - ot * A.group);
     const long long at =
         (static_cast<long long>(b) * A.sp.T + ot) * A.q_heads + oh;
     if (A.splits == 1) {
-      if (d < c.hd)
-        static_cast<uint16_t*>(A.out)[at * c.hd + d] =
-            E::from_f(sum == 0.0f ? 0.0f : o / sum);
+      put_row<E>(static_cast<uint16_t*>(A.out) + at * c.hd, d, c.hd, o, sum);
     } else {
-      A.partials[(at * A.splits + split) * HDP + d] = o;
+      *reinterpret_cast<f32x4*>(A.partials + (at * A.splits + split) * HDP +
+                                d) = o;
       if (d == 0) {
-        float* const st = A.stats + (at * A.splits + split) * 2;
-        st[0] = m;
-        st[1] = sum;
+        float* const s2 = A.stats + (at * A.splits + split) * 2;
+        s2[0] = m;
+        s2[1] = sum;
       }
     }
   }
@@ -1331,14 +1348,6 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
   const int clear = whole_wave ? (R.s.start + first + 1) / BLK : 0;
 
   if (R.lo < R.hi) {
-    h8 q[NR][NS];
-    float qscale[NR];
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      u16x8 raw[NS];
-      load_query<NS, E>(A, qrow[r], live[r], g, raw);
-      qscale[r] = query_fp16<NS, E>(A, raw, q[r]);
-    }
     const unsigned char* const kc =
         c.codes + static_cast<long long>(bh) * c.nblk * BLK * HDP;
     const float* const ksc = c.scales + static_cast<long long>(bh) * c.nblk;
@@ -1367,6 +1376,15 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
       if (lane < 2 * NE)
         scale_next = (lane < NE ? ksc : vsc)[min(blk + lane % NE, R.hi - 1)];
     };
+    load(R.lo);
+    h8 q[NR][NS];
+    float qscale[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      u16x8 raw[NS];
+      load_query<NS, E>(A, qrow[r], live[r], g, raw);
+      qscale[r] = query_fp16<NS, E>(A, raw, q[r]);
+    }
     ScaleRef<FP8> vs;
     // of the blocks in LDS: K's scale, what to multiply outputs with before
     // them, and V's scale against the reference
@@ -1396,7 +1414,6 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
         }
       }
     };
-    load(R.lo);
     store(0);
     __syncthreads();
     for (int blk = R.lo; blk < R.hi; blk += NE) {
@@ -1460,13 +1477,11 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
     for (int r = 0; r < NR; ++r) st[r].times(vs.ref);
   }
   if (R.tail) {
+    u16x8 raw[NR][NS];
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      u16x8 raw[NS];
-      load_query<NS, E>(A, qrow[r], live[r], g, raw);
-      tail_step<NS, E, false>(A, R, bh, lane, raw, seen[r],
-                       *reinterpret_cast<RowState<NS>(*)[1]>(&st[r]));
-    }
+    for (int r = 0; r < NR; ++r)
+      load_query<NS, E>(A, qrow[r], live[r], g, raw[r]);
+    tail_step<NS, NR, E>(A, R, bh, lane, raw, seen, st);
   }
 
 #pragma unroll
@@ -1483,12 +1498,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
       uint16_t* const out = static_cast<uint16_t*>(A.out) + at * c.hd;
 #pragma unroll
       for (int n = 0; n < 2 * NS; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int d = 16 * n + 4 * g + i;
-          if (d < c.hd)
-            out[d] = E::from_f(l == 0.0f ? 0.0f : st[r].o[n][i] / l);
-        }
+        put_row<E>(out, 16 * n + 4 * g, c.hd, st[r].o[n], l);
     } else {
       float* const part = A.partials + (at * A.splits + split) * HDP;
 #pragma unroll
@@ -1572,6 +1582,30 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(const float* partials,
     const float sum = s_sum;
     out[row * hd + d] = E::from_f(sum == 0.0f ? 0.0f : o / sum);
   }
+}
+
+// The same for many rows of few splits: a row of lanes each.
+template <int NS, typename E>
+__global__ __launch_bounds__(256) void kv8_join_rows_kernel(
+    const float* partials, const float* stats, uint16_t* out, long long rows,
+    int splits, int hd) {
+  constexpr int HDP = NS * 32, LANES = HDP / 4, GROUPS = 256 / LANES;
+  const int grp = threadIdx.x / LANES, d = threadIdx.x % LANES * 4;
+  const long long row = static_cast<long long>(blockIdx.x) * GROUPS + grp;
+  if (grp >= GROUPS || row >= rows) return;
+  const float* const st = stats + row * splits * 2;
+  const float* const p = partials + row * splits * HDP + d;
+  float top = kNone;
+  for (int s = 0; s < splits; ++s) top = fmaxf(top, st[2 * s]);
+  f32x4 o = {0, 0, 0, 0};
+  float sum = 0.0f;
+  for (int s = 0; s < splits; ++s) {
+    const float w = __builtin_amdgcn_exp2f(st[2 * s] - top);
+    o += *reinterpret_cast<const f32x4*>(p + static_cast<long long>(s) * HDP) *
+         w;
+    sum += w * st[2 * s + 1];
+  }
+  put_row<E>(out + row * hd, d, hd, o, sum);
 }
 
 // Heads that a row of lanes takes: as many as leave every CU six workgroups
@@ -1713,13 +1747,34 @@ extern "C" int fma_kv8_attn_splits(const FmaKv8Layer* c, int T, int q_heads,
   const long long groups =
       (rows + tile - 1) / tile * c->batch * c->kv_heads;
   const int nb = max_len / BLK;
-  // Four workgroups a CU (two of many rows), for sequences of different
-  // length to even out, and at least a block for each wave: 32 sequences of
-  // up to 8192 tokens, 8 kv heads, 1 / 2 / 4 / 8 / 16 splits took
-  // 74.0 / 61.5 / 58.1 / 60.0 / 66.4 us.
-  long long splits = groups > 0 ? (tile == 16 ? 4LL : 2LL) * cus / groups : 1;
-  if (splits > nb / 4) splits = nb / 4;
-  return splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : static_cast<int>(splits);
+  if (tile == 16) {
+    // Four workgroups a CU, for sequences of different length to even out,
+    // and at least a block for each wave: 32 sequences of up to 8192 tokens,
+    // 8 kv heads, 1 / 2 / 4 / 8 / 16 splits took 74.0 / 61.5 / 58.1 / 60.0 /
+    // 66.4 us.
+    long long splits = groups > 0 ? 4LL * cus / groups : 1;
+    if (splits > nb / 4) splits = nb / 4;
+    return splits < 1 ? 1
+           : splits > kMaxSplits ? kMaxSplits
+                                 : static_cast<int>(splits);
+  }
+  // Many rows: a workgroup's two blocks take about 1.1 us at a width of 128
+  // (two workgroups a CU at once); a join 3 us, and its rows written and read
+  // at 5 TB/s.
+  const double all = static_cast<double>(c->batch) * T * q_heads;
+  double best = 0.0;
+  int splits = 1;
+  for (int n = 1; n <= kMaxSplits && (n == 1 || n <= nb / 4); n *= 2) {
+    const double turns =
+        groups * n > 2LL * cus ? groups * n / (2.0 * cus) : 1.0;
+    const double us = nb / (2.0 * n) * turns * 1.1 * c->hdp / 128.0 +
+                      (n > 1 ? 3.0 + all * n * c->hdp * 8.0 / 5e6 : 0.0);
+    if (n == 1 || us < best) {
+      best = us;
+      splits = n;
+    }
+  }
+  return splits;
 }
 
 extern "C" hipError_t fma_launch_kv8_attention(FmaKv8Layer c, FmaKv8Span span,
@@ -1766,6 +1821,14 @@ extern "C" hipError_t fma_launch_kv8_attention(FmaKv8Layer c, FmaKv8Span span,
                      g, 256, 0, stream, a))));
   }
   if (err != hipSuccess || splits == 1) return err;
+  if (all >= 2048) {
+    FMA_BY_TYPE16(c.bf16, FMA_BY_WIDTH(c.hdp,
+        constexpr int GROUPS = 256 / (NS * 8);
+        return launch(kv8_join_rows_kernel<NS, E>,
+                      dim3(static_cast<unsigned>((all + GROUPS - 1) / GROUPS)),
+                      256, 0, stream, a.partials, a.stats,
+                      static_cast<uint16_t*>(out), all, splits, c.hd)));
+  }
   FMA_BY_TYPE16(c.bf16, FMA_BY_WIDTH(c.hdp,
       return launch(kv8_join_kernel<NS, E>, dim3(static_cast<unsigned>(all)),
                     256, 0, stream, a.partials, a.stats,
