@@ -1357,26 +1357,31 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
     // NE blocks of K and V, by way of registers. What lies behind the last
     // block comes as zeros, with that block's scales. Lane e of each wave
     // holds K's scale of block e, lane NE + e V's.
-    u32x4 kn[NE][EACH], vn[NE][EACH];
-    float scale_next = 0.0f;
-    auto load = [&](int blk) {
+    struct Staged {
+      u32x4 k[NE][EACH], v[NE][EACH];
+      float scale;
+    };
+    auto load = [&](Staged& to, int blk) {
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
         const long long at = static_cast<long long>(blk + e) * BLK * HDP;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
           const int u = threadIdx.x + i * 256;
-          kn[e][i] = vn[e][i] = u32x4{0, 0, 0, 0};
+          to.k[e][i] = to.v[e][i] = u32x4{0, 0, 0, 0};
           if ((UNITS % 256 == 0 || u < UNITS) && blk + e < R.hi) {
-            kn[e][i] = *reinterpret_cast<const u32x4*>(kc + at + u * 16);
-            vn[e][i] = *reinterpret_cast<const u32x4*>(vc + at + u * 16);
+            to.k[e][i] = *reinterpret_cast<const u32x4*>(kc + at + u * 16);
+            to.v[e][i] = *reinterpret_cast<const u32x4*>(vc + at + u * 16);
           }
         }
       }
       if (lane < 2 * NE)
-        scale_next = (lane < NE ? ksc : vsc)[min(blk + lane % NE, R.hi - 1)];
+        to.scale = (lane < NE ? ksc : vsc)[min(blk + lane % NE, R.hi - 1)];
     };
-    load(R.lo);
+    Staged one, two;
+    one.scale = two.scale = 0.0f;
+    load(one, R.lo);
+    if (R.lo + NE < R.hi) load(two, R.lo + NE);
     h8 q[NR][NS];
     float qscale[NR];
 #pragma unroll
@@ -1393,11 +1398,11 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
       return __uint_as_float(
           __builtin_amdgcn_readlane(__float_as_uint(x), i));
     };
-    auto store = [&](int buf) {
+    auto store = [&](const Staged& from, int buf) {
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
-        const float scale = lane_of(scale_next, NE + e);
-        kscale[e] = lane_of(scale_next, e);
+        const float scale = lane_of(from.scale, NE + e);
+        kscale[e] = lane_of(from.scale, e);
         more[e] = vs.follow(scale);
         ratio[e] = vs.ratio(scale);
 #pragma unroll
@@ -1405,7 +1410,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
           const int u = threadIdx.x + i * 256;
           if (UNITS % 256 == 0 || u < UNITS) {
             const int n = 2 * (u >> 6), l = u & 63;
-            const u32x4 a = kn[e][i], w = vn[e][i];
+            const u32x4 a = from.k[e][i], w = from.v[e][i];
             s_k[buf][e][n][l] = decode8(a[0], a[1], 1.0f, FP8);
             s_k[buf][e][n + 1][l] = decode8(a[2], a[3], 1.0f, FP8);
             s_v[buf][e][n][l] = decode8(w[0], w[1], ratio[e], FP8);
@@ -1414,11 +1419,11 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
         }
       }
     };
-    store(0);
+    store(one, 0);
     __syncthreads();
-    for (int blk = R.lo; blk < R.hi; blk += NE) {
-      const int buf = ((blk - R.lo) / NE) & 1;
-      if (blk + NE < R.hi) load(blk + NE);
+    // the blocks in LDS; `later` is filled with those after the next
+    auto step = [&](int blk, int buf, Staged& later, const Staged& next) {
+      if (blk + 2 * NE < R.hi) load(later, blk + 2 * NE);
       f32x4 x[NE][NR][2];
       float f[NE][NR];
 #pragma unroll
@@ -1470,8 +1475,12 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
                 vf, p[r], st[r].o[n], 0, 0, 0);
         }
       }
-      if (blk + NE < R.hi) store(buf ^ 1);
+      if (blk + NE < R.hi) store(next, buf ^ 1);
       __syncthreads();
+    };
+    for (int blk = R.lo; blk < R.hi; blk += 2 * NE) {
+      step(blk, 0, one, two);
+      if (blk + NE < R.hi) step(blk + NE, 1, two, one);
     }
 #pragma unroll
     for (int r = 0; r < NR; ++r) st[r].times(vs.ref);
