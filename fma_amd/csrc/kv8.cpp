@@ -266,18 +266,19 @@ class Kv8Buffers {
     const int max_len = span.start != nullptr
                             ? c.max_seq
                             : static_cast<int>(start_i) + span.T;
-    const int splits = fma_kv8_attn_splits(&c, span.T, q_heads, max_len,
-                                           compute_units(q.device().index()));
+    const FmaKv8Plan plan = fma_kv8_attn_plan(
+        &c, span.T, q_heads, max_len, compute_units(q.device().index()));
     at::Tensor partials;
     float* part = nullptr;
-    if (splits > 1) {
-      partials = at::empty({q.size(0) * q.size(1) * q_heads, splits, c.hdp + 2},
+    if (plan.splits > 1) {
+      partials = at::empty({q.size(0) * q.size(1) * q_heads, plan.splits,
+                            c.hdp + 2},
                            scales_.options());
       part = partials.data_ptr<float>();
     }
     KV8_HIP_CHECK(fma_launch_kv8_attention(c, span, qr, out.data_ptr(),
                                            q_heads, static_cast<float>(scale),
-                                           part, splits, stream.stream()));
+                                           part, plan, stream.stream()));
     return out;
   }
 

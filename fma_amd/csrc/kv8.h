@@ -82,11 +82,18 @@ extern "C" hipError_t fma_launch_kv8_read(FmaKv8Layer c, const int* start,
                                           int length_i, int n, void* ko,
                                           void* vo, hipStream_t stream);
 
+// How a call is spread: rows of one kv head that a workgroup takes, and parts
+// that the blocks of a sequence are split into.
+struct FmaKv8Plan {
+  int tile, splits;
+};
+// max_len: tokens that a sequence may have
+extern "C" FmaKv8Plan fma_kv8_attn_plan(const FmaKv8Layer* c, int T,
+                                        int q_heads, int max_len, int cus);
 // partials: fp32, rows * splits * (hdp + 2) of them where splits > 1
-extern "C" int fma_kv8_attn_splits(const FmaKv8Layer* c, int T, int q_heads,
-                                   int max_len, int cus);
 extern "C" hipError_t fma_launch_kv8_attention(FmaKv8Layer c, FmaKv8Span span,
                                                FmaRows q, void* out,
                                                int q_heads, float scale,
-                                               float* partials, int splits,
+                                               float* partials,
+                                               FmaKv8Plan plan,
                                                hipStream_t stream);

@@ -1739,57 +1739,66 @@ extern "C" hipError_t fma_launch_kv8_read(FmaKv8Layer c, const int* start,
 }
 
 namespace {
-// Rows of one kv head that a workgroup takes: 16 while they are few, then 64
-// times NR.
-constexpr int kFewRows = 32;
 constexpr int many_nr(int ns) { return ns <= 4 ? 2 : 1; }
 constexpr int many_ne(int ns) { return ns <= 4 ? 2 : 1; }
-int tile_rows(long long rows, int hdp) {
-  return rows <= kFewRows ? 16 : 64 * many_nr(hdp / 32);
-}
 }  // namespace
 
-extern "C" int fma_kv8_attn_splits(const FmaKv8Layer* c, int T, int q_heads,
-                                   int max_len, int cus) {
+extern "C" FmaKv8Plan fma_kv8_attn_plan(const FmaKv8Layer* c, int T,
+                                        int q_heads, int max_len, int cus) {
   const long long rows = static_cast<long long>(T) * (q_heads / c->kv_heads);
-  const int tile = tile_rows(rows, c->hdp);
-  const long long groups =
-      (rows + tile - 1) / tile * c->batch * c->kv_heads;
+  const long long heads = static_cast<long long>(c->batch) * c->kv_heads;
   const int nb = max_len / BLK;
-  if (tile == 16) {
+  const double wide = c->hdp / 128.0;
+  FmaKv8Plan plan;
+  // Tiles of 16 rows read the codes once each, so up to 64 rows they are taken
+  // while that is little: 8 kv heads of 128, 4000 tokens, 48 rows: 15.2 us
+  // against 19.2 us for one sequence, 37.1 against 35.9 us for eight (195 MB),
+  // 109 against 90 us for 32.
+  const double codes = 64.0 * nb * heads * c->hdp;
+  const long long few = (rows + 15) / 16;
+  if (few <= 1 || (few <= 4 && few * codes * wide <= 200e6)) {
+    plan.tile = 16;
     // Four workgroups a CU, for sequences of different length to even out,
     // and at least a block for each wave: 32 sequences of up to 8192 tokens,
     // 8 kv heads, 1 / 2 / 4 / 8 / 16 splits took 74.0 / 61.5 / 58.1 / 60.0 /
     // 66.4 us.
-    long long splits = groups > 0 ? 4LL * cus / groups : 1;
+    long long splits = few > 0 ? 4LL * cus / (few * heads) : 1;
     if (splits > nb / 4) splits = nb / 4;
-    return splits < 1 ? 1
-           : splits > kMaxSplits ? kMaxSplits
-                                 : static_cast<int>(splits);
+    plan.splits = splits < 1            ? 1
+                  : splits > kMaxSplits ? kMaxSplits
+                                        : static_cast<int>(splits);
+    return plan;
   }
-  // Many rows: a workgroup's two blocks take about 1.1 us at a width of 128
-  // (two workgroups a CU at once); a join 3 us, and its rows written and read
-  // at 5 TB/s.
+  // Many rows: what two blocks take a workgroup alone on its CU, and two of
+  // them together, as measured at widths 64 to 256; a join takes 3 us, and
+  // its rows are written and read at 5 TB/s.
+  plan.tile = 64 * many_nr(c->hdp / 32);
+  const double groups =
+      static_cast<double>((rows + plan.tile - 1) / plan.tile) * heads;
+  const double w = wide < 1.25 ? wide : 1.25;
   const double all = static_cast<double>(c->batch) * T * q_heads;
   double best = 0.0;
-  int splits = 1;
+  plan.splits = 1;
   for (int n = 1; n <= kMaxSplits && (n == 1 || n <= nb / 4); n *= 2) {
-    const double turns =
-        groups * n > 2LL * cus ? groups * n / (2.0 * cus) : 1.0;
-    const double us = nb / (2.0 * n) * turns * 1.1 * c->hdp / 128.0 +
+    const double turns = groups * n / (2.0 * cus);
+    const double pair = groups * n <= cus
+                            ? 1.0 + 0.8 * w
+                            : (0.5 + 1.6 * w) * (turns > 1.0 ? turns : 1.0);
+    const double us = nb / (2.0 * n) * pair +
                       (n > 1 ? 3.0 + all * n * c->hdp * 8.0 / 5e6 : 0.0);
     if (n == 1 || us < best) {
       best = us;
-      splits = n;
+      plan.splits = n;
     }
   }
-  return splits;
+  return plan;
 }
 
 extern "C" hipError_t fma_launch_kv8_attention(FmaKv8Layer c, FmaKv8Span span,
                                                FmaRows q, void* out,
                                                int q_heads, float scale,
-                                               float* partials, int splits,
+                                               float* partials,
+                                               FmaKv8Plan plan,
                                                hipStream_t stream) {
   if (c.batch == 0 || span.T == 0) return hipSuccess;
   AttnArgs a;
@@ -1799,14 +1808,14 @@ extern "C" hipError_t fma_launch_kv8_attention(FmaKv8Layer c, FmaKv8Span span,
   a.out = out;
   a.partials = partials;
   a.stats = partials + static_cast<long long>(c.batch) * span.T * q_heads *
-                           splits * c.hdp;
+                           plan.splits * c.hdp;
   a.scale = fmaxf(fabsf(scale) * kLog2e, 1.2e-38f);
   a.negative = scale < 0.0f;
   a.q_heads = q_heads;
   a.group = q_heads / c.kv_heads;
   const long long rows = static_cast<long long>(span.T) * a.group;
   const long long all = static_cast<long long>(c.batch) * span.T * q_heads;
-  const int tile = tile_rows(rows, c.hdp);
+  const int tile = plan.tile, splits = plan.splits;
   const long long tiles = (rows + tile - 1) / tile;
   const long long grid = tiles * c.batch * c.kv_heads * splits;
   if (rows > 0x7fffff00LL || all > 0x7fffffffLL || grid > 0x7fffffffLL)
