@@ -242,7 +242,8 @@ class Kv8Buffers {
 
   at::Tensor attention(const at::Tensor& q_in, int64_t layer,
                        const c10::optional<at::Tensor>& start, int64_t start_i,
-                       const c10::optional<at::Tensor>& counts, double scale) {
+                       const c10::optional<at::Tensor>& counts, double scale,
+                       int64_t held) {
     const FmaKv8Layer c = at_layer(layer);
     at::Tensor q = dense_last(q_in, "q");
     check_new(q, "q");
@@ -258,7 +259,11 @@ class Kv8Buffers {
     TORCH_CHECK_VALUE(q.size(2) >= 1 && q.size(2) % c.kv_heads == 0 &&
                     q.size(2) < (1 << 20),
                 "query heads must be a multiple of the cache's kv heads");
-    const FmaKv8Span span = span_of(q.size(1), start, start_i, counts);
+    FmaKv8Span span = span_of(q.size(1), start, start_i, counts);
+    TORCH_CHECK_VALUE(held == 0 || (held <= c.max_seq && span.start == nullptr &&
+                                    held >= start_i + q.size(1)),
+                      "tokens held do not fit the span");
+    span.held = static_cast<int>(held);
     c10::hip::HIPGuard guard(q.device().index());
     auto out = at::empty(q_in.sizes(), tail_.options());
     auto stream = c10::hip::getCurrentHIPStream(q.device().index());
@@ -389,5 +394,5 @@ void fma_bind_kv8(pybind11::module_& m) {
            py::arg("length_i"))
       .def("attention", &Kv8Buffers::attention, py::arg("q"),
            py::arg("layer"), py::arg("start"), py::arg("start_i"),
-           py::arg("counts"), py::arg("scale"));
+           py::arg("counts"), py::arg("scale"), py::arg("held"));
 }

@@ -995,11 +995,12 @@ __device__ inline h8 weights16(const f32x4 (&x)[2], float ratio) {
   return p;
 }
 
-// Where a tile of query rows reads its keys: its sequence, its blocks held as
-// codes, and whether it sees the incomplete block.
+// Where a tile of query rows reads its keys: its span, the tokens stored, the
+// blocks of them held as codes, those to read, and whether the tile sees the
+// incomplete one.
 struct Reach {
   Span s;
-  int full, lo, hi;
+  int held, full, lo, hi;
   bool tail;
 };
 __device__ inline Reach reach_of(const AttnArgs& A, int b, int row0, int rows,
@@ -1010,7 +1011,8 @@ __device__ inline Reach reach_of(const AttnArgs& A, int b, int row0, int rows,
   const int t_last =
       min((min(row0 + rows, A.rows) - 1) / A.group, r.s.count - 1);
   const int most = t_first < r.s.count ? r.s.start + t_last + 1 : 0;
-  r.full = r.s.end / BLK;
+  r.held = A.sp.held > 0 ? A.sp.held : r.s.end;
+  r.full = r.held / BLK;
   const long long nb = min(r.full, (most + BLK - 1) / BLK);
   r.lo = static_cast<int>(nb * split / A.splits);
   r.hi = static_cast<int>(nb * (split + 1) / A.splits);
@@ -1103,7 +1105,7 @@ __device__ inline void tail_step(const AttnArgs& A, const Reach& R, int bh,
       lo[r][i] = E::from_f(p - E::to_f(u));
     }
   }
-  const int held = R.s.end - R.full * BLK - 4 * g;
+  const int held = R.held - R.full * BLK - 4 * g;
 #pragma unroll
   for (int n = 0; n < 2 * NS; ++n) {
     u16x8 v = *reinterpret_cast<const u16x8*>(vt + (n >> 1) * 1024 +

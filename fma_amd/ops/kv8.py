@@ -256,7 +256,9 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, layer: int,
     start.. and are in the cache already, over everything up to themselves:
     softmax(scale * q K^T) V, scale = head_dim ** -0.5 by default, qH a
     multiple of kvH. start and counts as in :func:`kv8_append`; rows behind a
-    sequence's count come out as zeros."""
+    sequence's count come out as zeros. Where the cache knows its length the
+    queries may lie anywhere in it; else the span's last token has to be the
+    last one stored, which says what of it is coded already."""
     cache._check_layer(layer)
     given = isinstance(start, torch.Tensor)
     if not given:
@@ -265,8 +267,10 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, layer: int,
     if scale is None:
         scale = cache.head_dim ** -0.5
     if cache._native is not None:
+        held = None if given or counts is not None else cache._length[layer]
         return cache._native.attention(q, layer, start if given else None,
-                                       0 if given else start, counts, scale)
+                                       0 if given else start, counts, scale,
+                                       held or 0)
     cache._check_rows(q, "q", 0)
     cache._check_span(start, counts)
     return _attend(q, cache, layer, start, counts, scale)
@@ -275,9 +279,14 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, layer: int,
 def kv8_read(cache: KV8Cache, layer: int, start: Position, n: int,
              length: Position) -> Tuple[torch.Tensor, torch.Tensor]:
     """The keys and values [B, n, kvH, hd] that the cache stands for at
-    positions start..start+n-1 of sequences of ``length`` tokens, in its
-    16-bit type; zeros behind the length."""
+    positions start..start+n-1 of sequences of ``length`` tokens (all that
+    were stored: that says which are coded), in its 16-bit type; zeros behind
+    the length."""
     cache._check_layer(layer)
+    known = cache._length[layer]
+    if known is not None and not isinstance(length, torch.Tensor) \
+            and length != known:
+        raise ValueError(f"length {length}, but the cache holds {known}")
     if n < 0:
         raise ValueError(f"cannot read {n} tokens")
     args = []
@@ -407,8 +416,10 @@ def _attend(q: torch.Tensor, cache: KV8Cache, layer: int, start: Position,
         s, n = int(starts[b]), int(ns[b])
         if not n:
             continue
-        k, v = (x.repeat_interleave(group, 1).transpose(0, 1)
-                for x in _held(cache, layer, b, s + n))
+        known = None if counts is not None or isinstance(start, torch.Tensor) \
+            else cache._length[layer]
+        k, v = (x[:s + n].repeat_interleave(group, 1).transpose(0, 1)
+                for x in _held(cache, layer, b, known or s + n))
         v = torch.nan_to_num(v)
         score = q[b, :n].float().transpose(0, 1) @ k.transpose(1, 2) * scale
         late = torch.arange(s + n) > s + torch.arange(n)[:, None]

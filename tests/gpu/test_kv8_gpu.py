@@ -371,6 +371,154 @@ def test_attention_ignores_what_is_masked(ops):
                 oracle.check(out[b, :live], want, bound, BF)
 
 
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("T", [2, 40, 150])
+def test_attention_over_blocks_of_uneven_scale(ops, fmt, T):
+    """V's scale up and down by up to 2^40 from one block to the next, and
+    blocks of zeros, for few rows and for many."""
+    n = 500
+    k, v = randn(1, n, 2, 128), randn(1, n, 2, 128, seed=1)
+    for i, e in enumerate((0, 7, -7, 0, 20, 0, -13, -40, 0, 3, 9, -9, 6, -6,
+                           12, 0)):
+        v[:, 32 * i:32 * i + 32] *= 2.0 ** e
+    v[:, 160:192], k[:, 224:288] = 0, 0
+    c = ops.KV8Cache(2, 1, n, 2, 128, fmt=fmt, device="cuda")
+    ops.kv8_append(c, 1, k, v, 0)
+    q = randn(1, T, 8, 128, seed=2)
+    q[:, :, 3] *= 30                          # one block holds the row
+    attend_and_check(ops, c, q, k, v, n - T)
+
+
+@pytest.mark.parametrize("T,qh,kvh,n,B", [(200, 16, 1, 3300, 1),
+                                          (70, 12, 2, 4000, 1),
+                                          (1, 64, 2, 700, 32),
+                                          (12, 8, 2, 3000, 2)])
+def test_attention_splits_and_joins(ops, T, qh, kvh, n, B):
+    c, k, v = filled(ops, n, H=kvh, B=B, hd=64)
+    q = randn(B, T, qh, 64, seed=2)
+    attend_and_check(ops, c, q, k, v, n - T)
+
+
+def test_attention_scale_zero_is_the_mean(ops):
+    c, k, v = filled(ops, 100)
+    q = randn(1, 30, 8, 128, seed=2)
+    attend_and_check(ops, c, q, k, v, 70, scale=0.0)
+
+
+def test_queries_in_front_of_the_last_token(ops):
+    c, k, v = filled(ops, 150)
+    for start, T in ((49, 1), (40, 30), (0, 3), (127, 2), (95, 1), (20, 90)):
+        q = randn(1, T, 8, 128, seed=2)
+        out = ops.kv8_attention(q, c, 1, start)
+        n = start + T
+        want, bound = oracle.attention(
+            q[0], oracle.held(k[0], "fp8")[:n], oracle.held(v[0], "fp8")[:n],
+            start, 128 ** -0.5)
+        oracle.check(out[0], want, bound, BF)
+
+
+def test_capacity_inside_a_block(ops):
+    """max_seq 45: the last token, and tokens dropped behind it."""
+    c = ops.KV8Cache(2, 1, 45, 2, 128, device="cuda")
+    k, v = randn(1, 45, 2, 128), randn(1, 45, 2, 128, seed=1)
+    ops.kv8_append(c, 1, k, v, 0)
+    q = randn(1, 45, 8, 128, seed=2)
+    attend_and_check(ops, c, q, k, v, 0)
+    d = ops.KV8Cache(1, 1, 45, 2, 128, device="cuda")
+    wide = torch.cat((k, k), 1)
+    ops.kv8_append(d, 0, wide, torch.cat((v, v), 1), ints(0))
+    assert torch.equal(d.codes[0], c.codes[1])
+    for x, y in zip(ops.kv8_read(d, 0, 0, 45, ints(45)), (k, v)):
+        assert torch.equal(x[0].cpu(), value(oracle.held(y[0], "fp8"), BF))
+    out = ops.kv8_attention(randn(1, 90, 8, 128), d, 0, ints(0))
+    assert not out[:, 45:].any()
+
+
+def test_read_from_inside_a_block(ops):
+    c, k, v = filled(ops, 150, B=2)
+    for x, y in zip(ops.kv8_read(c, 1, 5, 100, 150), (k, v)):
+        assert torch.equal(x[1].cpu(), value(
+            oracle.held(y[1], "fp8")[5:105], BF))
+    got = ops.kv8_read(c, 1, ints(140, 3), 20, ints(150, 150))
+    for x, y in zip(got, (k, v)):
+        h = oracle.held(y[0], "fp8")
+        assert torch.equal(x[0, :10].cpu(), value(h[140:], BF))
+        assert not x[0, 10:].any()
+        h = oracle.held(y[1], "fp8")
+        assert torch.equal(x[1].cpu(), value(h[3:23], BF))
+
+
+def test_large_outputs_have_the_same_bits(ops):
+    """Outputs beyond the caches are stored past them."""
+    T = 5000
+    q, k, v = randn(1, T, 32, 128), randn(1, T, 8, 128), randn(1, T, 8, 128)
+    cos, sin = oracle.tables(T, 128, "cuda")
+    w = randn(128, seed=3)
+    got = ops.fast_qk_norm_rope(q, k, cos, sin, 0, w, w)
+    c, d = (ops.KV8Cache(1, 1, T, 8, 128, device="cuda") for _ in range(2))
+    qc = ops.qk_norm_rope_kv8(c, 0, q, k, v, cos, sin, 0, w, w)
+    assert torch.equal(qc, got[0])
+    for at in range(0, T, 800):
+        s = slice(at, at + 800)
+        part = ops.fast_qk_norm_rope(q[:, s], k[:, s], cos, sin, at, w, w)
+        assert torch.equal(part[0], got[0][:, s])
+        assert torch.equal(part[1], got[1][:, s])
+        ops.qk_norm_rope_kv8(d, 0, q[:, s], k[:, s], v[:, s], cos, sin, at, w,
+                             w)
+    assert torch.equal(c.codes, d.codes) and torch.equal(c.scales, d.scales)
+
+
+def test_refusals_on_the_gpu(ops):
+    """The same as on the CPU; nothing is launched."""
+    c, k, v = filled(ops, 10, cap=100)
+    cos, sin = oracle.tables(100, 128, "cuda")
+    q = randn(1, 1, 8, 128)
+    w = torch.ones(128, device="cuda", dtype=BF)
+    bad = [
+        lambda: ops.kv8_append(c, 2, k, v, 10),
+        lambda: ops.kv8_append(c, 1, k[..., :64], v, 10),
+        lambda: ops.kv8_append(c, 1, k.float(), v, 10),
+        lambda: ops.kv8_append(c, 1, k.cpu(), v, 10),
+        lambda: ops.kv8_append(c, 1, k, v[:, :5], 10),
+        lambda: ops.kv8_append(c, 1, k[:, :, :1], v[:, :, :1], 10),
+        lambda: ops.kv8_append(c, 1, k, v, 95),
+        lambda: ops.kv8_append(c, 1, k, v, -1),
+        lambda: ops.kv8_append(c, 1, k, v, 12),
+        lambda: ops.kv8_append(c, 1, k, v, ints(0, 0)),
+        lambda: ops.kv8_append(c, 1, k, v, torch.tensor([0], device="cuda")),
+        lambda: ops.kv8_append(c, 1, k, v, ints(0).cpu()),
+        lambda: ops.kv8_append(c, 1, k, v, 10, ints(1, 2)),
+        lambda: ops.kv8_append(c, 1, k.clone().requires_grad_(), v, 10),
+        lambda: ops.kv8_attention(q, c, 1, 10),
+        lambda: ops.kv8_attention(q[:, :, :3], c, 1, 9),
+        lambda: ops.kv8_attention(q.half(), c, 1, 9),
+        lambda: ops.kv8_attention(q.cpu(), c, 1, 9),
+        lambda: ops.kv8_attention(q[0], c, 1, 9),
+        lambda: ops.kv8_read(c, 1, 0, 5, 11),
+        lambda: ops.kv8_read(c, 1, 0, -1, 10),
+        lambda: ops.qk_norm_rope_kv8(c, 1, q, k, v, cos, sin, 10),
+        lambda: ops.qk_norm_rope_kv8(c, 1, q, k[:, :1], v[:, :1], cos[:99],
+                                     sin[:99], 10),
+        lambda: ops.fast_qk_norm_rope(q, q, cos, sin, 100),
+        lambda: ops.fast_qk_norm_rope(q, q, cos, sin[:50], 0),
+        lambda: ops.fast_qk_norm_rope(q, q, cos.half(), sin.half(), 0),
+        lambda: ops.fast_qk_norm_rope(q, q, cos, sin, 0, w[:64]),
+        lambda: ops.fast_qk_norm_rope(q, q, cos, sin, 0, w.float()),
+        lambda: ops.fast_qk_norm_rope(q, q, cos, sin, ints(0, 1)),
+        lambda: ops.fast_qk_norm_rope(q, q.half(), cos, sin, 0),
+        lambda: ops.fast_qk_norm_rope(q, k, cos, sin, 0),
+        lambda: ops.fast_qk_norm_rope(q.clone().requires_grad_(), q, cos, sin,
+                                      0),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was taken")
+    # the refused calls have changed nothing
+    ops.kv8_append(c, 1, k, v, 10)
+    assert torch.equal(ops.kv8_read(c, 1, 10, 10, 20)[0], k)
+
+
 def test_attention_nan_query_stays_in_its_row(ops):
     c, k, v = filled(ops, 90)
     q = randn(1, 20, 8, 128, seed=2)
@@ -489,6 +637,32 @@ def test_captured_steps_replay(ops):
         for out in outs:
             assert torch.equal(out, want), t
     torch.cuda.synchronize()
+
+
+def test_captured_attention_with_splits(ops):
+    """Split over a long axis inside a graph: positions change under it."""
+    B, H, cap = 2, 2, 4096
+    c = ops.KV8Cache(1, B, cap, H, 64, device="cuda")
+    k, v = randn(B, cap, H, 64), randn(B, cap, H, 64, seed=1)
+    q = randn(B, 1, 8, 64, seed=2)
+    start = ints(0, 0)
+    ops.kv8_append(c, 0, k, v, 0, counts=start + 1)
+    ops.kv8_attention(q, c, 0, start)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.kv8_attention(q, c, 0, start)
+    for ends in ((1, 4096), (4000, 77), (33, 32), (2048, 3000)):
+        ops.kv8_append(c, 0, k, v, 0, counts=ints(*ends))
+        start.copy_(ints(*ends) - 1)
+        g.replay()
+        eager = ops.kv8_attention(q, c, 0, start)
+        assert torch.equal(out, eager)
+        for b, n in enumerate(ends):
+            want, bound = oracle.attention(
+                q[b], oracle.held(k[b, :n], "fp8"),
+                oracle.held(v[b, :n], "fp8"), n - 1, 0.125)
+            oracle.check(out[b], want, bound, BF)
 
 
 def test_on_another_stream_and_twice_at_once(ops):

@@ -117,6 +117,20 @@ def test_attention_matches_the_oracle(fmt, T):
     oracle.check(out[0], want, bound, q.dtype)
 
 
+def test_queries_in_front_of_the_last_token():
+    k, v = kv(150)
+    c = make(S=200)
+    kv8_append(c, 0, k, v, 0)
+    for start, T in ((49, 1), (40, 30), (0, 3), (127, 2), (95, 1)):
+        q = torch.randn(1, T, 4, 16).bfloat16()
+        out = kv8_attention(q, c, 0, start)
+        n = start + T
+        want, bound = oracle.attention(
+            q[0], oracle.held(k[0], "fp8")[:n], oracle.held(v[0], "fp8")[:n],
+            start, 0.25)
+        oracle.check(out[0], want, bound, q.dtype)
+
+
 def test_ragged_batch():
     k, v = kv(50, B=3)
     c = make(B=3)
@@ -203,7 +217,8 @@ def test_refusals_of_the_cache():
                  (q.float(), c, 0, 9), (q[:, :, :1], c, 0, 9)):
         with pytest.raises(ValueError):
             kv8_attention(*args)
-    for args in ((0, 0, -1, 5), (0, 101, 1, 5), (0, 0, 1, 101)):
+    for args in ((0, 0, -1, 10), (0, 101, 1, 10), (0, 0, 1, 101),
+                 (0, 0, 1, 9)):
         with pytest.raises(ValueError):
             kv8_read(c, *args)
     c.free()
