@@ -280,8 +280,8 @@ def kv8_read(cache: KV8Cache, layer: int, start: Position, n: int,
              length: Position) -> Tuple[torch.Tensor, torch.Tensor]:
     """The keys and values [B, n, kvH, hd] that the cache stands for at
     positions start..start+n-1 of sequences of ``length`` tokens (all that
-    were stored: that says which are coded), in its 16-bit type; zeros behind
-    the length."""
+    were stored: that says which are coded), in its 16-bit type, where they
+    saturate; zeros behind the length."""
     cache._check_layer(layer)
     known = cache._length[layer]
     if known is not None and not isinstance(length, torch.Tensor) \
@@ -311,7 +311,11 @@ def kv8_read(cache: KV8Cache, layer: int, start: Position, n: int,
         m = min(n, end - s)
         if m > 0:
             for w, x in enumerate(_held(cache, layer, b, end)):
-                out[w, b, :m] = x[s:s + m].to(cache.dtype)
+                top = torch.finfo(cache.dtype).max
+                coded = max(min(end // BLOCK * BLOCK - s, m), 0)
+                x = x[s:s + m]
+                out[w, b, :coded] = x[:coded].clamp(-top, top).to(cache.dtype)
+                out[w, b, coded:m] = x[coded:].to(cache.dtype)
     return out[0], out[1]
 
 

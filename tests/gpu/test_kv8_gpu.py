@@ -233,6 +233,17 @@ def test_scales_at_the_ends_of_the_types(ops):
             rk, rv = ops.kv8_read(c, 0, 0, 32, 32)
             assert torch.equal(rk[0].cpu(), value(oracle.held(k[0], fmt), BF))
             assert torch.equal(rv, -rk)
+    # a code may stand for more than the type holds: it saturates
+    for dtype in (BF, HF):
+        k = torch.full((1, 32, 1, 64), torch.finfo(dtype).max, device="cuda",
+                       dtype=dtype)
+        c = ops.KV8Cache(1, 1, 32, 1, 64, dtype=dtype, device="cuda")
+        d = ops.KV8Cache(1, 1, 32, 1, 64, dtype=dtype)
+        ops.kv8_append(c, 0, k, -k, 0)
+        ops.kv8_append(d, 0, k.cpu(), -k.cpu(), 0)
+        rk, rv = ops.kv8_read(c, 0, 0, 32, 32)
+        assert torch.equal(rk, k) and torch.equal(rv, -k)
+        assert torch.equal(ops.kv8_read(d, 0, 0, 32, 32)[0], k.cpu())
 
 
 @pytest.mark.parametrize("interleaved", [True, False])
