@@ -968,8 +968,8 @@ __device__ inline void settle(const f32x4 (&x)[NE][NR][2],
     for (int r = 0; r < NR; ++r) st[r].refer(top[r], more);
   }
 }
-// x becomes the weights; their sum is advanced.
-template <int NS>
+// x becomes the weights; their sum is advanced where SUM.
+template <int NS, bool SUM>
 __device__ inline void weigh(f32x4 (&x)[2], float f, RowState<NS>& st) {
   float sum = 0.0f;
 #pragma unroll
@@ -977,9 +977,9 @@ __device__ inline void weigh(f32x4 (&x)[2], float f, RowState<NS>& st) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       x[a][i] = __builtin_amdgcn_exp2f(fmaf(x[a][i], f, -st.m));
-      sum += x[a][i];
+      if (SUM) sum += x[a][i];
     }
-  st.l += sum;
+  if (SUM) st.l += sum;
 }
 // left: how many of the lane's tokens on are seen
 __device__ inline void mask(f32x4 (&x)[2], int left) {
@@ -1107,7 +1107,7 @@ __device__ inline void tail_step(const AttnArgs& A, const Reach& R, int bh,
   u16x8 hi[NR], lo[NR];
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
-    weigh<NS>(x[0][r], A.scale, st[r]);
+    weigh<NS, true>(x[0][r], A.scale, st[r]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float p = x[0][r][i >> 2][i & 3];
@@ -1252,7 +1252,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
       const float f[1][1] = {{factor(kscale, qscale)}};
       mask(x, seen - blk * BLK - 4 * g);
       settle<NS, 1, 1>(xs, f, state, vs.follow(vscale));
-      weigh<NS>(x, f[0][0], st);
+      weigh<NS, true>(x, f[0][0], st);
       const float ratio = vs.ratio(vscale);
       const h8 p = weights16<FP8>(x, ratio);
 #pragma unroll
@@ -1403,6 +1403,12 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
       load_query<NS, E>(A, qrow[r], live[r], g, raw);
       qscale[r] = query_fp16<NS, E>(A, raw, q[r]);
     }
+    // Where the weights are not scaled the matrix unit sums them, as one more
+    // row of V^T: 16 additions less for the other. l is then the row's whole
+    // sum in each lane.
+    h8 ones;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ones[i] = static_cast<_Float16>(1.0f);
     ScaleRef<FP8> vs;
     // of the blocks in LDS: K's scale, what to multiply outputs with before
     // them, and V's scale against the reference
@@ -1467,7 +1473,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
                  blk + e < R.hi ? seen[r] - (blk + e) * BLK - 4 * g : 0);
       }
       // Of two waves on a SIMD the one that is further goes first, so that
-      // they do not wait for the same unit: 545 us against 565 us.
+      // they do not wait for the same unit: 443 us against 467 us.
       __builtin_amdgcn_s_setprio(1);
       settle<NS, NR, NE>(x, f, st, more[0]);
 #pragma unroll
@@ -1479,9 +1485,13 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
         h8 p[NR];
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-          weigh<NS>(x[e][r], f[e][r], st[r]);
+          weigh<NS, !FP8>(x[e][r], f[e][r], st[r]);
           p[r] = weights16<FP8>(x[e][r], ratio[e]);
+          if (FP8)
+            st[r].l = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                ones, p[r], f32x4{st[r].l, 0, 0, 0}, 0, 0, 0)[0];
         }
+        __builtin_amdgcn_s_setprio(2);
 #pragma unroll
         for (int n = 0; n < 2 * NS; ++n) {
           const h8 vf = s_v[buf][e][n][lane];
@@ -1491,8 +1501,8 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
                 vf, p[r], st[r].o[n], 0, 0, 0);
         }
       }
-      __builtin_amdgcn_s_setprio(0);
       if (blk + NE < R.hi) store(next, buf ^ 1);
+      __builtin_amdgcn_s_setprio(0);
       __syncthreads();
     };
     for (int blk = R.lo; blk < R.hi; blk += 2 * NE) {
@@ -1500,7 +1510,10 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
       if (blk + NE < R.hi) step(blk + NE, 1, two, one);
     }
 #pragma unroll
-    for (int r = 0; r < NR; ++r) st[r].times(vs.ref);
+    for (int r = 0; r < NR; ++r) {
+      st[r].times(vs.ref);
+      if (FP8) st[r].l *= 0.25f;  // this lane's share again
+    }
   }
   if (R.tail) {
     u16x8 raw[NR][NS];
