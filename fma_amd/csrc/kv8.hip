@@ -1796,22 +1796,31 @@ extern "C" FmaKv8Plan fma_kv8_attn_plan(const FmaKv8Layer* c, int T,
   const double wide = c->hdp / 128.0;
   FmaKv8Plan plan;
   // Tiles of 16 rows read the codes once each, so up to 64 rows they are taken
-  // while that is little: 8 kv heads of 128, 4000 tokens, 48 rows: 15.2 us
-  // against 19.2 us for one sequence, 37.1 against 35.9 us for eight (195 MB),
-  // 109 against 90 us for 32.
+  // while that is little: 8 kv heads of 128, 4000 tokens, 48 rows: 12.2 us
+  // against 19.2 us for one sequence, 37.0 against 35.9 us for eight (195 MB),
+  // 109 against 85 us for 32.
   const double codes = 64.0 * nb * heads * c->hdp;
   const long long few = (rows + 15) / 16;
   if (few <= 1 || (few <= 4 && few * codes * wide <= 200e6)) {
     plan.tile = 16;
-    // Four workgroups a CU, for sequences of different length to even out,
-    // and at least a block for each wave: 32 sequences of up to 8192 tokens,
-    // 8 kv heads, 1 / 2 / 4 / 8 / 16 splits took 74.0 / 61.5 / 58.1 / 60.0 /
-    // 66.4 us.
-    long long splits = few > 0 ? 4LL * cus / (few * heads) : 1;
-    if (splits > nb / 4) splits = nb / 4;
-    plan.splits = splits < 1            ? 1
-                  : splits > kMaxSplits ? kMaxSplits
-                                        : static_cast<int>(splits);
+    // A join costs 2.5 us, so short axes stay whole (heads of 128, 8 kv heads,
+    // one sequence: 24 blocks 7.5 us whole, 7.7 us in eight; 32 blocks 8.6 and
+    // 7.8 us). Then a workgroup for each CU while each has four blocks; and
+    // four for each CU, for sequences of different length to even out, while
+    // each has 16: eight sequences of 4095 tokens in 1 / 4 / 8 / 16 parts 30.4
+    // / 17.1 / 15.0 / 17.0 us; 32 of up to 8192 in 1 / 2 / 4 / 8 / 16 parts
+    // 74.0 / 61.5 / 58.1 / 60.0 / 66.4 us.
+    const long long all = few * heads;
+    plan.splits = 1;
+    if (all > 0 && nb > (c->hdp <= 128 ? 24 : 16)) {
+      const long long one = cus / all < nb / 4 ? cus / all : nb / 4;
+      const long long four = 4LL * cus / all < nb / 16 ? 4LL * cus / all
+                                                       : nb / 16;
+      const long long most = one > four ? one : four;
+      plan.splits = most < 1            ? 1
+                    : most > kMaxSplits ? kMaxSplits
+                                        : static_cast<int>(most);
+    }
     return plan;
   }
   // Many rows: what two blocks take a workgroup alone on its CU, and two of
