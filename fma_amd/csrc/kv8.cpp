@@ -89,6 +89,9 @@ FmaRope rope_of(const c10::optional<at::Tensor>& cos,
   }
   auto weight = [&](const c10::optional<at::Tensor>& w) -> const void* {
     if (!w.has_value()) return nullptr;
+    TORCH_CHECK_VALUE(!(w->requires_grad() && at::GradMode::is_enabled()),
+                      "a norm weight requires a gradient; there is no backward "
+                      "pass");
     TORCH_CHECK_VALUE(w->device() == like.device() &&
                     w->scalar_type() == like.scalar_type() &&
                     w->numel() == hd && w->is_contiguous(),
@@ -240,6 +243,15 @@ class Kv8Buffers {
     return {ko, vo};
   }
 
+  // Whether a call now would be recorded. The default stream cannot be.
+  bool capturing() const {
+    hipStream_t stream =
+        c10::hip::getCurrentHIPStream(codes_.device().index()).stream();
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (stream != nullptr) KV8_HIP_CHECK(hipStreamIsCapturing(stream, &status));
+    return status != hipStreamCaptureStatusNone;
+  }
+
   at::Tensor attention(const at::Tensor& q_in, int64_t layer,
                        const c10::optional<at::Tensor>& start, int64_t start_i,
                        const c10::optional<at::Tensor>& counts, double scale,
@@ -260,9 +272,8 @@ class Kv8Buffers {
                     q.size(2) < (1 << 20),
                 "query heads must be a multiple of the cache's kv heads");
     FmaKv8Span span = span_of(q.size(1), start, start_i, counts);
-    TORCH_CHECK_VALUE(held == 0 || (held <= c.max_seq && span.start == nullptr &&
-                                    held >= start_i + q.size(1)),
-                      "tokens held do not fit the span");
+    TORCH_CHECK_VALUE(held >= 0 && held <= c.max_seq,
+                      "tokens held beyond the cache");
     span.held = static_cast<int>(held);
     c10::hip::HIPGuard guard(q.device().index());
     auto out = at::empty(q_in.sizes(), tail_.options());
@@ -389,6 +400,7 @@ void fma_bind_kv8(pybind11::module_& m) {
            py::arg("cos"), py::arg("sin"), py::arg("start"),
            py::arg("start_i"), py::arg("q_norm"), py::arg("k_norm"),
            py::arg("counts"), py::arg("eps"), py::arg("pairs"))
+      .def("capturing", &Kv8Buffers::capturing)
       .def("read", &Kv8Buffers::read, py::arg("layer"), py::arg("start"),
            py::arg("start_i"), py::arg("n"), py::arg("length"),
            py::arg("length_i"))

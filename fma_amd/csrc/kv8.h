@@ -34,7 +34,7 @@ struct FmaKv8Span {
   const int* counts;
   int start_i;
   int T;
-  int held;  // tokens stored of every sequence; 0: as many as the span ends at
+  int held;  // tokens stored of every sequence, if not only those of the span
 };
 
 // Rows of a [B, T, H, hd] tensor with a contiguous last dimension.

@@ -1028,7 +1028,7 @@ __device__ inline Reach reach_of(const AttnArgs& A, int b, int row0, int rows,
   const int t_last =
       min((min(row0 + rows, A.rows) - 1) / A.group, r.s.count - 1);
   const int most = t_first < r.s.count ? r.s.start + t_last + 1 : 0;
-  r.held = A.sp.held > 0 ? A.sp.held : r.s.end;
+  r.held = max(A.sp.held, r.s.end);
   r.full = r.held / BLK;
   const long long nb = min(r.full, (most + BLK - 1) / BLK);
   r.lo = static_cast<int>(nb * split / A.splits);

@@ -83,6 +83,9 @@ def _check_rope(q, k, cos, sin, q_norm, k_norm) -> None:
                               or not w.is_contiguous()):
             raise ValueError(f"norm weights must be contiguous {q.dtype} "
                              f"[{hd}] on {q.device}")
+        if w is not None and w.requires_grad and torch.is_grad_enabled():
+            raise ValueError("a norm weight requires a gradient; this has no "
+                             "backward pass")
 
 
 def rope_rows(x, w, cos, sin, pos, eps: float, interleaved: bool):

@@ -45,8 +45,10 @@ class KV8Cache:
 
     Where positions are given as numbers the cache follows each layer's
     length and refuses calls that would leave a hole or build on values it no
-    longer holds; where they live on the GPU the caller answers for that, and
-    tokens outside [0, max_seq) are dropped.
+    longer holds; where they live on the GPU the caller answers for that,
+    tokens behind max_seq are dropped, and so are all of a sequence whose
+    position is negative. The same holds for a layer that a captured graph
+    appends to, whose replays the host does not see.
     """
 
     def __init__(self, num_layers: int, batch: int, max_seq: int,
@@ -75,6 +77,8 @@ class KV8Cache:
         self.tail = torch.zeros((*lead, 2, BLOCK * self.width), dtype=dtype,
                                 device=device)
         self.device = self.codes.device
+        # layers without a store that a graph repeats
+        self._followed = [True] * num_layers
         self._native = None
         if self.device.type == "cuda":
             self._native = actuation.require_native().Kv8Buffers(
@@ -82,10 +86,15 @@ class KV8Cache:
                 fmt == "fp8")
         self.reset()
 
+    def _check_scale(self, scale: float) -> None:
+        if not abs(scale) < 3.4e38:
+            raise ValueError(f"scale must be finite in fp32, got {scale}")
+
     def reset(self) -> None:
         """Forget all tokens (nothing is cleared)."""
         # None: appended at positions that only the GPU knows
-        self._length: List[Optional[int]] = [0] * self.num_layers
+        self._length: List[Optional[int]] = [
+            0 if followed else None for followed in self._followed]
         self._raw_from = [0] * self.num_layers
 
     @property
@@ -160,7 +169,10 @@ class KV8Cache:
                 counts: Optional[torch.Tensor]) -> None:
         if not T:
             return
-        if counts is not None or isinstance(start, torch.Tensor):
+        if self._native is not None and self._native.capturing():
+            self._followed[layer] = False
+        if counts is not None or isinstance(start, torch.Tensor) \
+                or not self._followed[layer]:
             self._length[layer] = None
             return
         known, end = self._length[layer], start + T
@@ -257,8 +269,9 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, layer: int,
     softmax(scale * q K^T) V, scale = head_dim ** -0.5 by default, qH a
     multiple of kvH. start and counts as in :func:`kv8_append`; rows behind a
     sequence's count come out as zeros. Where the cache knows its length the
-    queries may lie anywhere in it; else the span's last token has to be the
-    last one stored, which says what of it is coded already."""
+    queries may lie anywhere in it; else, and in a captured graph, each
+    sequence's last query has to be the last token stored, which says what of
+    it is coded already."""
     cache._check_layer(layer)
     given = isinstance(start, torch.Tensor)
     if not given:
@@ -266,8 +279,16 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, layer: int,
                    counts)
     if scale is None:
         scale = cache.head_dim ** -0.5
+    cache._check_scale(scale)
     if cache._native is not None:
-        held = None if given or counts is not None else cache._length[layer]
+        held = cache._length[layer]
+        if held is not None and cache._native.capturing():
+            # the length at a replay is not today's
+            if not given and counts is None and start + q.shape[1] != held:
+                raise ValueError(
+                    f"a captured call's queries must end at the last of the "
+                    f"{held} tokens held")
+            held = None
         return cache._native.attention(q, layer, start if given else None,
                                        0 if given else start, counts, scale,
                                        held or 0)
@@ -420,10 +441,9 @@ def _attend(q: torch.Tensor, cache: KV8Cache, layer: int, start: Position,
         s, n = int(starts[b]), int(ns[b])
         if not n:
             continue
-        known = None if counts is not None or isinstance(start, torch.Tensor) \
-            else cache._length[layer]
         k, v = (x[:s + n].repeat_interleave(group, 1).transpose(0, 1)
-                for x in _held(cache, layer, b, known or s + n))
+                for x in _held(cache, layer, b,
+                               max(cache._length[layer] or 0, s + n)))
         v = torch.nan_to_num(v)
         score = q[b, :n].float().transpose(0, 1) @ k.transpose(1, 2) * scale
         late = torch.arange(s + n) > s + torch.arange(n)[:, None]

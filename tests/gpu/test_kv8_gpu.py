@@ -757,3 +757,91 @@ def test_tables_of_a_model_longer_than_its_cache():
     assert out.shape == (3, 50)
     with pytest.raises(ValueError, match="tables"):
         eng.model.forward(toks, eng.new_kv_cache(3, 300), 0)
+
+
+def test_padded_queries_in_front_of_the_last_token(ops):
+    c, k, v = filled(ops, 150, B=2, hd=64, cap=200)
+    for start, T, counts in ((10, 4, (3, 1)), (0, 150, (150, 40)),
+                             (97, 40, (2, 40))):
+        q = randn(2, T, 8, 64, seed=T)
+        n, s = ints(*counts), ints(start, start)
+        outs = [ops.kv8_attention(q, c, 1, start, n),
+                ops.kv8_attention(q, c, 1, s, n), ops.kv8_attention(q, c, 1, s)]
+        for i, out in enumerate(outs):
+            for b, m in enumerate(counts if i < 2 else (T, T)):
+                want, bound = oracle.attention(
+                    q[b, :m], oracle.held(k[b], "fp8")[:start + m],
+                    oracle.held(v[b], "fp8")[:start + m], start, 0.125)
+                oracle.check(out[b, :m], want, bound, BF)
+                assert not out[b, m:].any()
+
+
+def test_gradients_of_gains_and_bad_scales_are_refused(ops):
+    q = randn(1, 2, 2, 64)
+    cos, sin = oracle.tables(10, 64, "cuda")
+    w = torch.ones(64, device="cuda", dtype=BF, requires_grad=True)
+    c, k, v = filled(ops, 3, hd=64, cap=10)
+    for args in ((w, None), (None, w)):
+        with pytest.raises(ValueError, match="gradient"):
+            ops.fast_qk_norm_rope(q, q, cos, sin, 0, *args)
+        with pytest.raises(ValueError, match="gradient"):
+            ops.qk_norm_rope_kv8(c, 1, q, q, q, cos, sin, 3, *args)
+        with torch.no_grad():
+            ops.fast_qk_norm_rope(q, q, cos, sin, 0, *args)
+    for scale in (float("nan"), float("inf"), -1e300):
+        with pytest.raises(ValueError, match="scale"):
+            ops.kv8_attention(q[:, :1], c, 1, 2, scale=scale)
+
+
+def test_captured_calls_and_lengths_that_the_host_knows(ops):
+    """Replays move the cache without the host: what it knew before them does
+    not count, and a captured call does not keep what it knew."""
+    B, H, cap = 1, 2, 256
+    c = ops.KV8Cache(1, B, cap, H, 64, device="cuda")
+    k, v = randn(B, cap, H, 64), randn(B, cap, H, 64, seed=1)
+    q = randn(B, 1, 4, 64, seed=2)
+    at = ints(60)
+    kb, vb = torch.zeros_like(k[:, :1]), torch.zeros_like(v[:, :1])
+
+    def check(out, n):
+        want, bound = oracle.attention(q[0], oracle.held(k[0, :n], "fp8"),
+                                       oracle.held(v[0, :n], "fp8"), n - 1,
+                                       0.125)
+        oracle.check(out[0], want, bound, BF)
+
+    # attention alone: recorded while the host knows the length, replayed at
+    # other ones
+    ops.kv8_append(c, 0, k[:, :100], v[:, :100], 0)
+    ops.kv8_attention(q, c, 0, at)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.kv8_attention(q, c, 0, at)
+        with pytest.raises(ValueError, match="captured"):
+            ops.kv8_attention(q, c, 0, 60)
+    for n in (100, 61, 200, 96, 130):
+        ops.kv8_append(c, 0, k[:, :n], v[:, :n], 0)
+        at.fill_(n - 1)
+        g.replay()
+        check(out, n)
+        check(ops.kv8_attention(q, c, 0, at), n)
+    # a recorded store: the host knew 40 tokens, replays add 30
+    ops.kv8_append(c, 0, k[:, :40], v[:, :40], 0)
+    at.fill_(40)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.kv8_append(c, 0, kb, vb, at)
+        out = ops.kv8_attention(q, c, 0, at)
+    for _ in range(2):
+        c.reset()
+        ops.kv8_append(c, 0, k[:, :40], v[:, :40], 0)
+        for t in range(40, 70):
+            at.fill_(t)
+            kb.copy_(k[:, t:t + 1])
+            vb.copy_(v[:, t:t + 1])
+            g.replay()
+            check(out, t + 1)
+        # by number behind the replays
+        ops.kv8_append(c, 0, k[:, 70:75], v[:, 70:75], 70)
+        check(ops.kv8_attention(q, c, 0, 74), 75)

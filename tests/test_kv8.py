@@ -341,3 +341,44 @@ def test_option_reaches_the_engine():
     cfg.dtype = torch.float32
     with pytest.raises(ValueError):
         ActuationEngine(cfg, kv_cache_dtype="fp8")
+
+
+def test_padded_queries_in_front_of_the_last_token():
+    """Counts and a tensor of starts say nothing of what is coded where the
+    cache knows its length."""
+    k, v = kv(150, B=2)
+    c = make(S=200, B=2)
+    kv8_append(c, 0, k, v, 0)
+    for start, T, counts in ((10, 4, (3, 1)), (0, 150, (150, 40)),
+                             (97, 40, (2, 40))):
+        q = torch.randn(2, T, 4, 16).bfloat16()
+        n = torch.tensor(counts, dtype=torch.int32)
+        s = torch.full((2,), start, dtype=torch.int32)
+        outs = [kv8_attention(q, c, 0, start, n),
+                kv8_attention(q, c, 0, s, n)]
+        outs.append(kv8_attention(q, c, 0, s))
+        for i, out in enumerate(outs):
+            for b, m in enumerate(counts if i < 2 else (T, T)):
+                want, bound = oracle.attention(
+                    q[b, :m], oracle.held(k[b], "fp8")[:start + m],
+                    oracle.held(v[b], "fp8")[:start + m], start, 0.25)
+                oracle.check(out[b, :m], want, bound, q.dtype)
+                assert not out[b, m:].any()
+
+
+def test_gradients_of_gains_and_bad_scales_are_refused():
+    q, k = torch.randn(1, 2, 2, 8), torch.randn(1, 2, 1, 8)
+    cos, sin = oracle.tables(10, 8)
+    w = torch.ones(8, requires_grad=True)
+    for args in ((w, None), (None, w)):
+        with pytest.raises(ValueError, match="gradient"):
+            fast_qk_norm_rope(q, k, cos, sin, 0, *args)
+        with torch.no_grad():
+            fast_qk_norm_rope(q, k, cos, sin, 0, *args)
+    c = make()
+    kk, v = kv(3)
+    kv8_append(c, 0, kk, v, 0)
+    one = torch.zeros(1, 1, 2, 16).bfloat16()
+    for scale in (float("nan"), float("inf"), -1e300):
+        with pytest.raises(ValueError, match="scale"):
+            kv8_attention(one, c, 0, 2, scale=scale)
