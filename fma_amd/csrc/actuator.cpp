@@ -1490,6 +1490,20 @@ at::Tensor attn_prefill_bf16(const at::Tensor& q, const at::Tensor& k,
   return out;
 }
 
+// hipHostFree waits for what is on its way.
+at::Tensor alloc_pinned(int64_t nbytes) {
+  TORCH_CHECK_VALUE(nbytes >= 1, "cannot pin ", nbytes, " bytes");
+  void* p = nullptr;
+  const hipError_t err = hipHostMalloc(&p, static_cast<size_t>(nbytes),
+                                       hipHostMallocDefault);
+  if (err != hipSuccess) (void)hipGetLastError();  // reported here, once
+  TORCH_CHECK(err == hipSuccess, "cannot pin ", nbytes, " bytes of host memory: ",
+              hipGetErrorString(err));
+  return at::from_blob(
+      p, {nbytes}, [](void* q) { (void)hipHostFree(q); },
+      at::TensorOptions().dtype(at::kByte));
+}
+
 std::tuple<int64_t, int64_t> device_mem_info(int device) {
   FMA_HIP_CHECK(hipSetDevice(device));
   size_t free_b = 0, total_b = 0;
@@ -1558,6 +1572,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "Batched gather kernel D2D microbench (returns seconds/iteration)",
         py::arg("tensors"), py::arg("offsets"), py::arg("out"),
         py::arg("repeats") = 1);
+  m.def("alloc_pinned", &alloc_pinned, "Pinned host bytes, not rounded up",
+        py::arg("nbytes"));
   m.def("device_mem_info", &device_mem_info, py::arg("device"));
   fma_bind_kv8(m);
   py::class_<DeviceArena>(m, "DeviceArena")

@@ -103,8 +103,12 @@ def plan_layout(specs: Sequence[Tuple[str, Tuple[int, ...], torch.dtype]],
 def alloc_pinned(nbytes: int) -> torch.Tensor:
     """One pinned host buffer. Allocated once per instance and reused across
     every sleep/wake cycle (pinning cost stays off the wake path). Plain
-    host memory on GPU-less machines (tests)."""
+    host memory on GPU-less machines (tests). Torch's allocator rounds to a
+    power of two, 128 GiB for a model of 64.75, so a large buffer is
+    allocated at its own size."""
     if torch.cuda.is_available():
+        if nbytes >= 1 << 30 and native_available():
+            return _C.alloc_pinned(nbytes)
         return torch.empty(nbytes, dtype=torch.uint8, pin_memory=True)
     return torch.empty(nbytes, dtype=torch.uint8)
 

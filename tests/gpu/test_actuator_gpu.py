@@ -737,3 +737,17 @@ def test_attn_prefill16_matches_fp32_reference():
                  (out.float() - ref).abs().max().item())
     finally:
         os.environ.pop("FMA_PREFILL_16", None)
+
+
+def test_large_pinned_buffer_is_not_rounded_up():
+    from fma_amd.ops.actuation import alloc_pinned
+    n = (1 << 30) + (1 << 29) + 4097       # torch would pin 2 GiB
+    host = alloc_pinned(n)
+    assert host.is_pinned() and host.dtype == torch.uint8
+    assert host.untyped_storage().nbytes() == n
+    dev = torch.arange(4097, device="cuda").to(torch.uint8)
+    host[-4097:].copy_(dev, non_blocking=True)
+    torch.cuda.synchronize()
+    assert torch.equal(host[-4097:], dev.cpu())
+    assert torch.equal(host[-4097:].to("cuda", non_blocking=True), dev)
+    torch.cuda.synchronize()
