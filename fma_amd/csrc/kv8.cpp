@@ -228,7 +228,7 @@ class Kv8Buffers {
       int64_t layer, const c10::optional<at::Tensor>& start, int64_t start_i,
       int64_t n, const c10::optional<at::Tensor>& length, int64_t length_i) {
     const FmaKv8Layer c = at_layer(layer);
-    TORCH_CHECK_VALUE(n >= 0 && n < (1 << 30) && start_i >= 0 &&
+    TORCH_CHECK_VALUE(n >= 0 && n < (1 << 29) && start_i >= 0 &&
                     start_i < (1 << 30) && length_i >= 0 &&
                     length_i <= c.max_seq,
                 "range outside the cache");

@@ -726,7 +726,8 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(
   const int j = blockIdx.x % blocks;
   const int bh = blockIdx.x / blocks;
   const int b = bh / c.kv_heads, h = bh - b * c.kv_heads;
-  const int s0 = max(start != nullptr ? start[b] : start_i, 0);
+  // behind max_seq all is zero
+  const int s0 = min(max(start != nullptr ? start[b] : start_i, 0), c.max_seq);
   int len = length != nullptr ? length[b] : length_i;
   len = min(max(len, 0), c.max_seq);
   const int blk = s0 / BLK + j;

@@ -308,7 +308,7 @@ def kv8_read(cache: KV8Cache, layer: int, start: Position, n: int,
     if known is not None and not isinstance(length, torch.Tensor) \
             and length != known:
         raise ValueError(f"length {length}, but the cache holds {known}")
-    if n < 0:
+    if not 0 <= n < 1 << 29:
         raise ValueError(f"cannot read {n} tokens")
     args = []
     for value, name in ((start, "start"), (length, "length")):

@@ -845,3 +845,28 @@ def test_captured_calls_and_lengths_that_the_host_knows(ops):
         # by number behind the replays
         ops.kv8_append(c, 0, k[:, 70:75], v[:, 70:75], 70)
         check(ops.kv8_attention(q, c, 0, 74), 75)
+
+
+def test_read_from_far_behind_the_cache(ops):
+    c, k, _ = filled(ops, 40, B=3, hd=64, cap=64)
+    junk = [torch.full((1 << 20,), 7.0, device="cuda") for _ in range(4)]
+    del junk                                # what outputs would lie in
+    start = ints(2 ** 31 - 1, -5, 2 ** 31 - 40)
+    rk, rv = ops.kv8_read(c, 1, start, 70, 40)
+    assert not rk[0].any() and not rk[2].any()
+    assert not rv[0].any() and not rv[2].any()
+    assert torch.equal(rk[1, 32:40], k[1, 32:]) and not rk[1, 40:].any()
+
+
+def test_positions_far_outside_store_and_see_nothing(ops):
+    c, k, v = filled(ops, 40, B=3, hd=64, cap=64)
+    before = [x.clone() for x in (c.codes, c.scales, c.tail)]
+    far = ints(2 ** 31 - 1, -2 ** 31, 65)
+    ops.kv8_append(c, 1, k, v, far)
+    assert all(torch.equal(a, b)
+               for a, b in zip(before, (c.codes, c.scales, c.tail)))
+    for T in (1, 40):
+        q = randn(3, T, 8, 64, seed=T)
+        assert not ops.kv8_attention(q, c, 1, far).any()
+        assert not ops.kv8_attention(q, c, 1, far, ints(T, 2 ** 31 - 1,
+                                                        -2 ** 31)).any()
