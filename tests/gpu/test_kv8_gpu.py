@@ -870,3 +870,28 @@ def test_positions_far_outside_store_and_see_nothing(ops):
         assert not ops.kv8_attention(q, c, 1, far).any()
         assert not ops.kv8_attention(q, c, 1, far, ints(T, 2 ** 31 - 1,
                                                         -2 ** 31)).any()
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("hd", [160, 192, 256])
+@pytest.mark.parametrize("T,n", [(33, 64), (70, 500), (150, 501), (200, 2700)])
+def test_attention_wide_heads(ops, fmt, hd, T, n):
+    """Many rows at widths over 128: scores that grow from block to block, in
+    either half of a block or in both, for some rows; V's scale up and down."""
+    k, v = randn(1, n, 2, hd), randn(1, n, 2, hd, seed=1)
+    for i in range(0, n, 32):
+        v[:, i:i + 32] *= 2.0 ** ((0, 7, -7, 20, 0, -13, 3, -9)[i // 32 % 8])
+    q = randn(1, T, 8, hd, seed=2)
+    for j, at in enumerate(range(5, n, 23)):  # now in one half, now the other
+        k[:, at] = (q[:, T // 2, 1::4] * min(0.3 * (j + 1), 6)).to(BF)
+    q[:, :, 2] *= 25
+    q[:, 3, 6] = float("nan")
+    c = ops.KV8Cache(2, 1, n, 2, hd, fmt=fmt, device="cuda")
+    ops.kv8_append(c, 1, k, v, 0)
+    out = ops.kv8_attention(q, c, 1, n - T)
+    assert torch.isnan(out[0, 3, 6]).all()
+    q[:, 3, 6] = 0
+    again = attend_and_check(ops, c, q, k, v, n - T)
+    out[0, 3, 6] = again[0, 3, 6]
+    assert torch.equal(out, again)
+    attend_and_check(ops, c, q[:, :, :2], k, v, n - T, scale=-0.2)
