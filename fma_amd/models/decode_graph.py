@@ -27,8 +27,7 @@ import torch.nn.functional as F
 
 from fma_amd.ops.decode_ops import (available as _fused_available,
                                     fast_rope_qkv_store,
-                                    fast_rmsnorm, fast_rope1,
-                                    fast_silu_mul)
+                                    fast_rmsnorm, fast_rope1)
 from fma_amd.ops.kv8 import kv8_attention, qk_norm_rope_kv8
 from fma_amd.ops.linear import (fast_linear, fast_linear_multi,
                                 fast_linear_residual)
@@ -50,18 +49,23 @@ class StaticDecoder:
     """Single-token decode with static shapes over a private KV cache."""
 
     @staticmethod
-    def supported(cfg, kv_cache_dtype: str = "auto") -> bool:
+    def supported(cfg, kv_cache_dtype: str = "auto",
+                  any_vocab: bool = False) -> bool:
+        """Whether the step computes this model (``any_vocab``: whatever a
+        captured one may hold)."""
         # MoE routing is data-dependent per token: un-capturable;
         # qk_norm (qwen3) is outside the fused qkv+rope capture set, but
         # inside the 8-bit cache's one-launch norm + rope + store
-        if cfg.vocab_size > GRAPH_SAFE_VOCAB or cfg.num_experts:
+        if cfg.num_experts or (cfg.qk_norm and kv_cache_dtype == "auto"):
             return False
-        if kv_cache_dtype != "auto":
-            return cfg.hidden_act == "silu" and not cfg.embed_scale
-        return not cfg.qk_norm
+        return any_vocab or cfg.vocab_size <= GRAPH_SAFE_VOCAB
 
     def __init__(self, model: LlamaModel, batch: int, max_seq: int):
         assert model.tp_size == 1, "graphed decode is single-rank for now"
+        if not self.supported(model.cfg, model.kv_cache_dtype, True):
+            raise ValueError(f"the static step does not compute "
+                             f"{model.cfg.name}: experts, or q/k norms over "
+                             f"a 16-bit cache")
         self.model = model
         self.cfg = model.cfg
         self.batch = batch
@@ -106,6 +110,8 @@ class StaticDecoder:
         hd = cfg.head_dim
 
         x = F.embedding(self.input_tok, P["embed.weight"])  # [B,1,H]
+        if cfg.embed_scale:
+            x = x * (cfg.hidden_size ** 0.5)
         cos = m.rope_cos.index_select(0, self.pos.view(1))  # [1, hd/2]
         sin = m.rope_sin.index_select(0, self.pos.view(1))
         # graph-safe fused attention: the kernel reads t from this device
@@ -189,14 +195,14 @@ class StaticDecoder:
                 h = fast_rmsnorm(x, P[p + "mlp_norm.weight"], cfg.norm_eps)
                 gate, up = fast_linear_multi(
                     h, (P[p + "w_gate.weight"], P[p + "w_up.weight"]))
-                x = fast_linear_residual(fast_silu_mul(gate, up),
+                x = fast_linear_residual(m._act(gate, up, True),
                                          P[p + "w_down.weight"], x)
             else:
                 x = x + fast_linear(att, P[p + "wo.weight"])
                 h = fast_rmsnorm(x, P[p + "mlp_norm.weight"], cfg.norm_eps)
                 gate = fast_linear(h, P[p + "w_gate.weight"])
                 up = fast_linear(h, P[p + "w_up.weight"])
-                x = x + fast_linear(fast_silu_mul(gate, up),
+                x = x + fast_linear(m._act(gate, up, True),
                                     P[p + "w_down.weight"])
 
         x = fast_rmsnorm(x, P["final_norm.weight"], cfg.norm_eps)

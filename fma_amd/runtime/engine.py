@@ -263,7 +263,8 @@ class ActuationEngine:
     def _graph_decoder(self, batch: int, need_seq: int):
         """Lazily built hipGraph decoder for batch-1 serving (2.5x on
         launch-bound models, ~parity on HBM-bound ones; selection via
-        FMA_GRAPH_DECODE=1/0/auto). Dropped on sleep: its KV cache holds
+        FMA_GRAPH_DECODE=1/0/auto; 1 lifts the vocabulary limit, not what
+        the step can compute). Dropped on sleep: its KV cache holds
         HBM the sleep must release, and the captured kernel args point at
         arena slabs that wake re-allocates — replaying a pre-sleep graph
         after wake would read freed memory. Rebuilt + recaptured at the
@@ -273,7 +274,8 @@ class ActuationEngine:
                 or not self.on_gpu):
             return None
         from fma_amd.models.decode_graph import StaticDecoder as _SD
-        if mode != "1" and not _SD.supported(self.cfg, self.kv_cache_dtype):
+        if not _SD.supported(self.cfg, self.kv_cache_dtype,
+                             any_vocab=mode == "1"):
             # measured ROCm 7.2 graph-replay fault at large vocab
             # (decode_graph.GRAPH_SAFE_VOCAB); eager decode is clean
             return None

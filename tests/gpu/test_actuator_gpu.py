@@ -751,3 +751,29 @@ def test_large_pinned_buffer_is_not_rounded_up():
     assert torch.equal(host[-4097:], dev.cpu())
     assert torch.equal(host[-4097:].to("cuda", non_blocking=True), dev)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("kv", ["auto", "fp8"])
+def test_engine_graph_decode_of_gelu_and_scaled_embeddings(kv):
+    from fma_amd.models.llama import LlamaConfig
+    from fma_amd.runtime.engine import ActuationEngine
+    cfg = LlamaConfig(name="ggelu", vocab_size=512, hidden_size=512,
+                      intermediate_size=768, num_layers=2, num_heads=4,
+                      num_kv_heads=2, max_seq_len=128,
+                      hidden_act="gelu_tanh", embed_scale=True)
+    eng = ActuationEngine(cfg, 0, seed=7, kv_cache_dtype=kv)
+    toks = torch.arange(3, 20, device="cuda:0")[None]
+    want = eng.model.generate(toks, 20)
+    for _ in range(3):
+        assert torch.equal(eng.generate(toks, 20), want)
+    assert eng.stats()["graph_decode"] is True
+
+
+def test_graph_decode_override_keeps_to_what_the_step_computes(monkeypatch):
+    from fma_amd.models.llama import LlamaConfig
+    from fma_amd.runtime.engine import ActuationEngine
+    monkeypatch.setenv("FMA_GRAPH_DECODE", "1")
+    eng = ActuationEngine(LlamaConfig.tiny_qwen3(), 0, seed=7)
+    toks = torch.arange(3, 20, device="cuda:0")[None]
+    assert torch.equal(eng.generate(toks, 8), eng.model.generate(toks, 8))
+    assert eng.stats()["graph_decode"] is False

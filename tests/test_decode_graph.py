@@ -57,3 +57,27 @@ def test_graph_decoder_gated_on_safe_vocab():
     qwen = LlamaConfig.by_name("qwen2-7b")
     assert qwen.vocab_size > GRAPH_SAFE_VOCAB
     assert not StaticDecoder.supported(qwen)
+
+
+@pytest.mark.parametrize("kv", ["auto", "fp8", "int8"])
+def test_static_decode_of_gelu_and_scaled_embeddings(kv):
+    """The step has the model's activation and the embedding's factor."""
+    eng = ActuationEngine(LlamaConfig.tiny_gemma(), seed=5, kv_cache_dtype=kv)
+    prompt = torch.arange(3, 24)[None]
+    assert StaticDecoder.supported(eng.cfg, kv)
+    dec = StaticDecoder(eng.model, batch=1, max_seq=64)
+    assert torch.equal(dec.generate(prompt, 30),
+                       eng.model.generate(prompt, 30))
+
+
+def test_static_decoder_refuses_what_its_step_leaves_out():
+    """Whatever the vocabulary limit is overridden with."""
+    for cfg, kv in ((LlamaConfig.tiny_qwen3(), "auto"),
+                    (LlamaConfig.tiny_moe(), "auto"),
+                    (LlamaConfig.tiny_moe(), "fp8")):
+        assert not StaticDecoder.supported(cfg, kv, any_vocab=True)
+        eng = ActuationEngine(cfg, seed=5, kv_cache_dtype=kv)
+        with pytest.raises(ValueError, match="does not compute"):
+            StaticDecoder(eng.model, batch=1, max_seq=32)
+    assert StaticDecoder.supported(LlamaConfig.by_name("qwen2-7b"),
+                                   any_vocab=True)
