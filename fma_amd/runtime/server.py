@@ -37,7 +37,7 @@ from typing import List, Optional
 from fastapi import FastAPI, Query
 from fastapi.responses import JSONResponse
 
-from fma_amd.models.llama import LlamaConfig
+from fma_amd.models.llama import LlamaConfig, check_kv_cache_dtype
 
 
 def parse_options(options: str) -> argparse.Namespace:
@@ -55,7 +55,8 @@ def parse_options(options: str) -> argparse.Namespace:
     ap.add_argument("--served-model-name", default=None)
     ap.add_argument("--start-asleep", action="store_true",
                     help="immediately sleep after load (pre-warmed instance)")
-    ap.add_argument("--kv-cache-dtype", default="auto",
+    ap.add_argument("--kv-cache-dtype", default="auto", nargs="?",
+                    const="auto",
                     help="auto (the model's type), fp8 / fp8_e4m3 or int8: "
                          "hold keys and values in 8 bits")
     args, unknown = ap.parse_known_args(options.split())
@@ -70,6 +71,17 @@ def parse_options(options: str) -> argparse.Namespace:
         # node agent / launcher export the Pod's loopback identity
         args.host = os.environ.get("FMA_BIND_HOST", "0.0.0.0")
     return args
+
+
+def kv_cache_dtype_for(cfg: LlamaConfig, wanted: str) -> str:
+    """``wanted``, or "auto" with a note where an 8-bit cache cannot hold
+    this model's heads: the option never keeps a model from being served."""
+    try:
+        return check_kv_cache_dtype(cfg, wanted)
+    except ValueError as e:
+        print(f"[serve] --kv-cache-dtype {wanted}: {e}; using auto",
+              flush=True)
+        return "auto"
 
 
 def _free_port() -> int:
@@ -103,7 +115,8 @@ def _worker_entry(rank: int, world: int, master_port: int,
                           tp_rank=rank, tp_size=world,
                           tp_group=ctx.device_group, seed=seed,
                           init_weights=checkpoint is None,
-                          kv_cache_dtype=kv_cache_dtype)
+                          kv_cache_dtype=kv_cache_dtype_for(
+                              cfg, kv_cache_dtype))
     if checkpoint:
         eng.load_checkpoint(checkpoint)
     tp.run_worker_loop(ctx, eng)
@@ -182,8 +195,9 @@ class ServingRuntime:
                                  tp_rank=0, tp_size=world,
                                  tp_group=ctx.device_group, seed=args.seed,
                                  init_weights=checkpoint is None,
-                                 kv_cache_dtype=getattr(
-                                     args, "kv_cache_dtype", "auto"))
+                                 kv_cache_dtype=kv_cache_dtype_for(
+                                     cfg, getattr(args, "kv_cache_dtype",
+                                                  "auto")))
         if checkpoint is not None:
             t_load = engine.load_checkpoint(checkpoint)
             print(f"[serve] checkpoint {checkpoint} loaded in {t_load:.2f}s",

@@ -382,3 +382,24 @@ def test_gradients_of_gains_and_bad_scales_are_refused():
     for scale in (float("nan"), float("inf"), -1e300):
         with pytest.raises(ValueError, match="scale"):
             kv8_attention(one, c, 0, 2, scale=scale)
+
+
+def test_option_does_not_keep_a_model_from_being_served(monkeypatch, capsys):
+    """Heads that no 8-bit cache holds, and an option without a value."""
+    from fma_amd.models.llama import LlamaConfig
+    from fma_amd.runtime.server import ServingRuntime, parse_options
+    args = parse_options("--model tiny --kv-cache-dtype --seed 3")
+    assert (args.kv_cache_dtype, args.seed) == ("auto", 3)
+
+    def wide(name):
+        cfg = LlamaConfig.tiny()
+        cfg.head_dim_override = 288
+        return cfg
+    monkeypatch.setattr(LlamaConfig, "by_name", staticmethod(wide))
+    rt = ServingRuntime(parse_options("--model tiny --kv-cache-dtype int8"))
+    try:
+        assert rt.rt.stats()["kv_cache_dtype"] == "auto"
+        assert "using auto" in capsys.readouterr().out
+        assert len(rt.rt.generate_text("hello", 3)) >= 0
+    finally:
+        rt.close()
