@@ -1572,8 +1572,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "Batched gather kernel D2D microbench (returns seconds/iteration)",
         py::arg("tensors"), py::arg("offsets"), py::arg("out"),
         py::arg("repeats") = 1);
+  // pinning 64 GiB takes a second: other threads of the server go on
   m.def("alloc_pinned", &alloc_pinned, "Pinned host bytes, not rounded up",
-        py::arg("nbytes"));
+        py::arg("nbytes"), py::call_guard<py::gil_scoped_release>());
   m.def("device_mem_info", &device_mem_info, py::arg("device"));
   fma_bind_kv8(m);
   py::class_<DeviceArena>(m, "DeviceArena")

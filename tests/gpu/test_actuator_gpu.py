@@ -777,3 +777,29 @@ def test_graph_decode_override_keeps_to_what_the_step_computes(monkeypatch):
     toks = torch.arange(3, 20, device="cuda:0")[None]
     assert torch.equal(eng.generate(toks, 8), eng.model.generate(toks, 8))
     assert eng.stats()["graph_decode"] is False
+
+
+def test_pinning_lets_other_threads_run():
+    """A server answers while an instance's buffer is pinned."""
+    import threading
+    import time
+    from fma_amd.ops.actuation import alloc_pinned
+    alloc_pinned(1 << 30)                  # everything loaded and set up
+    stop, ticks = threading.Event(), []
+
+    def tick():
+        while not stop.wait(0.001):
+            ticks.append(time.perf_counter())
+    th = threading.Thread(target=tick)
+    th.start()
+    time.sleep(0.02)
+    t0 = time.perf_counter()
+    host = alloc_pinned(8 << 30)
+    t1 = time.perf_counter()
+    stop.set()
+    th.join()
+    assert host.numel() == 8 << 30
+    during = sum(t0 < t < t1 for t in ticks)
+    # 1 ms each if nothing holds them up; a call that keeps the interpreter
+    # to itself leaves room for one at each end
+    assert during >= min(20, (t1 - t0) / 0.01), (during, t1 - t0)
