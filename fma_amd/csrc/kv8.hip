@@ -821,10 +821,17 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(
 //
 // K and V are made fp16 on the way into the matrix unit: e4m3 and int8 fit
 // exactly. A query row is scaled by a power of two to fit fp16, exactly but
-// for values 2^24 below the row's largest. The weights are rounded to fp16
-// (half a step is 2^-11 of each, against 2^-8 of the bf16 result). A block's
-// K scale multiplies its scores; its V scale relative to a running reference
-// goes into V's conversion (fp8: a power of two, exact) or the weights (int8).
+// for values 2^24 below the row's largest. The weights are rounded to fp16:
+// half a step is 2^-11 of each, against 2^-8 of a bf16 result and as much as
+// an fp16 result's own, where a row has no more than a few tokens for it to
+// even out over. So that this holds for small weights too, a row's largest
+// stands at 2^7 or more (int8: 2^6): down to 2^-21 (2^-20) of the largest a
+// weight has all of its bits, and below it is off by at most 2^-32 (2^-31) of
+// the largest. With the largest at 1, 16384 tokens of 2^-26 beside one that
+// holds the row, which first tokens of real models do, all came out as zero.
+// A block's K scale multiplies its scores; its V scale relative to a running
+// reference goes into V's conversion (fp8: a power of two, exact) or the
+// weights (int8).
 
 __device__ inline h8 decode8(uint32_t lo, uint32_t hi, float scale, bool fp8) {
   h2 a, b, cc, d;
@@ -885,14 +892,16 @@ __device__ inline float row_max(float x) {
 }
 
 // The running reference of V's scales. It moves where fp16 has no room for
-// the ratio to it; down only as far as fp32 sums cannot overflow.
+// the ratio to it; down only as far as fp32 sums cannot overflow. Beside the
+// weights (int8) there is room for a ratio of 2.
 template <bool FP8>
 struct ScaleRef {
+  static constexpr uint32_t kUp = FP8 ? 6 : 1;
   float ref = 0.0f, inv = 0.0f, most = 0.0f;
   // a difference of bits is one of exponents, to a part of one
   __device__ bool far(float scale) const {
     return static_cast<uint32_t>(__float_as_int(scale) - __float_as_int(ref) +
-                                 (6 << 23)) > (12u << 23);
+                                 (6 << 23)) > ((6 + kUp) << 23);
   }
   // moves it where need be; returns what to multiply outputs with
   __device__ float follow(float scale) {
@@ -918,9 +927,13 @@ struct ScaleRef {
 // its own: its weights are exp2(-inf) and its factors multiply zeros.
 constexpr float kNone = -3e38f;
 
-// One wave's softmax and output state for 16 query rows.
-template <int NS>
+// One wave's softmax and output state for 16 query rows. The reference stands
+// LEAD (log2) below the largest score that it was taken from, and moves when
+// one passes it by MOST: weights go up to 2^15, times 2 where V's ratio is
+// beside them.
+template <int NS, bool FP8>
 struct RowState {
+  static constexpr float LEAD = FP8 ? 7.0f : 6.0f, MOST = LEAD + 8.0f;
   f32x4 o[2 * NS];  // O^T in units of vref: value 16 n + 4 g + reg, row l % 16
   float m, l;       // running reference and this lane's share of the sum
   __device__ void clear() {
@@ -937,7 +950,7 @@ struct RowState {
   }
   __device__ void refer(float top, float more) {
     top = row_max(top);
-    const float next = top > m + 8.0f ? top : m;
+    const float next = top > m + MOST ? top - LEAD : m;
     const float g = exp2f(m - next);
     m = next;
     l *= g;
@@ -946,13 +959,13 @@ struct RowState {
 };
 
 // x: products of NE blocks with NR times 16 rows; f > 0: what makes them log2
-// scores. A row's reference moves only when a score passes it by 2^8, which
+// scores. A row's reference moves only when a score has grown by 2^8, which
 // fp16 weights and fp32 sums have room for: the outputs are rarely rescaled,
 // and while no lane asks for it, no value has to cross lanes.
 // more: what the outputs are to be multiplied with in any case.
-template <int NS, int NR, int NE>
+template <int NR, int NE, typename RS>
 __device__ inline void settle(const f32x4 (&x)[NE][NR][2],
-                              const float (&f)[NE][NR], RowState<NS> (&st)[NR],
+                              const float (&f)[NE][NR], RS (&st)[NR],
                               float more) {
   float top[NR];
   bool grows = false;
@@ -968,7 +981,7 @@ __device__ inline void settle(const f32x4 (&x)[NE][NR][2],
       y *= f[e][r];
       top[r] = e == 0 ? y : __builtin_elementwise_maximum(top[r], y);
     }
-    grows |= top[r] > st[r].m + 8.0f;
+    grows |= top[r] > st[r].m + RS::MOST;
   }
   if (__any(grows) || more != 1.0f) {
 #pragma unroll
@@ -976,8 +989,8 @@ __device__ inline void settle(const f32x4 (&x)[NE][NR][2],
   }
 }
 // x becomes the weights; their sum is advanced where SUM.
-template <int NS, bool SUM>
-__device__ inline void weigh(f32x4 (&x)[2], float f, RowState<NS>& st) {
+template <bool SUM, typename RS>
+__device__ inline void weigh(f32x4 (&x)[2], float f, RS& st) {
   float sum = 0.0f;
 #pragma unroll
   for (int a = 0; a < 2; ++a)
@@ -1075,11 +1088,11 @@ __device__ inline float query_fp16(const AttnArgs& A, const u16x8 (&raw)[NS],
 
 // The incomplete block, raw, for NR times 16 rows. Its weights go in as two
 // 16-bit parts: a single bf16 would cost as much as the result's rounding.
-template <int NS, int NR, typename E>
+template <int NS, int NR, typename E, bool FP8>
 __device__ inline void tail_step(const AttnArgs& A, const Reach& R, int bh,
                                  int lane, const u16x8 (&q)[NR][NS],
                                  const int (&seen)[NR],
-                                 RowState<NS> (&st)[NR]) {
+                                 RowState<NS, FP8> (&st)[NR]) {
   const int g = lane >> 4;
   const uint16_t* const kt =
       static_cast<const uint16_t*>(A.c.tail) +
@@ -1110,11 +1123,11 @@ __device__ inline void tail_step(const AttnArgs& A, const Reach& R, int bh,
     }
     mask(x[0][r], seen[r] - R.full * BLK - 4 * g);
   }
-  settle<NS, NR, 1>(x, f, st, 1.0f);
+  settle<NR, 1>(x, f, st, 1.0f);
   u16x8 hi[NR], lo[NR];
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
-    weigh<NS, true>(x[0][r], A.scale, st[r]);
+    weigh<true>(x[0][r], A.scale, st[r]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float p = x[0][r][i >> 2][i & 3];
@@ -1199,8 +1212,8 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
   const bool live = row < A.rows && t < R.s.count;
   const int seen = live ? R.s.start + t + 1 : 0;  // keys of this row
 
-  RowState<NS> state[1];
-  RowState<NS>& st = state[0];
+  RowState<NS, FP8> state[1];
+  RowState<NS, FP8>& st = state[0];
   st.clear();
 
   if (R.lo < R.hi || R.tail) {
@@ -1261,8 +1274,8 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
       }
       const float f[1][1] = {{factor(kscale, qscale)}};
       mask(x, seen - blk * BLK - 4 * g);
-      settle<NS, 1, 1>(xs, f, state, vs.follow(vscale));
-      weigh<NS, true>(x, f[0][0], st);
+      settle<1, 1>(xs, f, state, vs.follow(vscale));
+      weigh<true>(x, f[0][0], st);
       const float ratio = vs.ratio(vscale);
       const h8 p = weights16<FP8>(x, ratio);
 #pragma unroll
@@ -1353,7 +1366,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
   constexpr int ROWS = 64 * NR;
   const Reach R = reach_of(A, b, tile * ROWS, ROWS, split);
 
-  RowState<NS> st[NR];
+  RowState<NS, FP8> st[NR];
   int seen[NR];
   const uint16_t* qrow[NR];
   bool live[NR];
@@ -1490,7 +1503,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
       // Of two waves on a SIMD the one that is further goes first, so that
       // they do not wait for the same unit: 443 us against 467 us.
       __builtin_amdgcn_s_setprio(1);
-      settle<NS, NR, NE>(x, f, st, more[0]);
+      settle<NR, NE>(x, f, st, more[0]);
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
         if (e > 0 && more[e] != 1.0f) {
@@ -1500,7 +1513,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
         h8 p[NR];
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-          weigh<NS, !FP8>(x[e][r], f[e][r], st[r]);
+          weigh<!FP8>(x[e][r], f[e][r], st[r]);
           p[r] = weights16<FP8>(x[e][r], ratio[e]);
           if (FP8)
             st[r].l = __builtin_amdgcn_mfma_f32_16x16x32_f16(

@@ -895,3 +895,35 @@ def test_attention_wide_heads(ops, fmt, hd, T, n):
     out[0, 3, 6] = again[0, 3, 6]
     assert torch.equal(out, again)
     attend_and_check(ops, c, q[:, :, :2], k, v, n - T, scale=-0.2)
+
+
+# -- small weights beside one that holds the row ------------------------------
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("B,T,n,H,group", [(2, 1, 773, 2, 8),
+                                           (1, 1024, 1024, 32, 1),
+                                           (1, 40, 5000, 2, 4)])
+def test_attention_first_token_holds_the_rows(ops, fmt, B, T, n, H, group):
+    """The first token, whose V is zero, has 2^26 times the weight of each
+    other: what the others give has to come out."""
+    hd = 64
+    scale = hd ** -0.5
+    base = randn(1, 1, H, hd, dtype=FP)
+    k = randn(B, n, H, hd, dtype=FP, seed=1) * 0.2
+    k[:, :1] = base * (18.0 / scale) / base.square().sum(-1, keepdim=True)
+    v = 1 + 0.1 * randn(B, n, H, hd, dtype=FP, seed=2)
+    v[:, 0] = 0
+    k, v = k.to(BF), v.to(BF)
+    q = (base.repeat_interleave(group, 2)
+         * (1 + 0.05 * randn(B, T, H * group, 1, dtype=FP, seed=3))).to(BF)
+    c = ops.KV8Cache(2, B, n, H, hd, fmt=fmt, device="cuda")
+    ops.kv8_append(c, 1, k, v, 0)
+    out = ops.kv8_attention(q, c, 1, n - T)
+    for b in range(B):
+        want, bound = oracle.attention_tight(
+            q[b], oracle.held(k[b], fmt), oracle.held(v[b], fmt), n - T,
+            scale, 2.0 ** (-32 if fmt == "fp8" else -30))
+        # the bound says something: the smaller part of what is looked for
+        last = (bound[-1] / want[-1].abs()).max()
+        assert last < 0.6, last
+        oracle.check(out[b], want, bound, BF)

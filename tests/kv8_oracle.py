@@ -69,6 +69,34 @@ def attention(q, k, v, start, scale):
     return out.transpose(0, 1), bound.transpose(0, 1)
 
 
+def attention_tight(q, k, v, start, scale, step):
+    """As :func:`attention`, with a bound that knows that a weight under
+    2^-20 of the row's largest is off by at most `step` of it: for each token
+    that the row sees, times that token's own largest value (the cache's
+    kernel for that: 2^-32 fp8, 2^-31 int8; a V scale may lie 2 under the
+    reference of the others, so int8 tests give 2^-30)."""
+    out, _ = attention(q, k, v, start, scale)
+    q, k, v = q.double().cpu(), k.double().cpu(), v.double().cpu()
+    T, n = q.shape[0], k.shape[0]
+    group = q.shape[1] // k.shape[1]
+    k = k.repeat_interleave(group, 1).permute(1, 2, 0)
+    v = v.repeat_interleave(group, 1).transpose(0, 1).abs()
+    qt = q.transpose(0, 1)
+    late = torch.arange(n) > start + torch.arange(T)[:, None]
+    s = (qt @ k * scale).masked_fill(late, float("-inf"))
+    p = torch.softmax(s, -1)
+    size = p @ v
+    ds = 2.0 ** -24 * q.shape[2] * (qt.abs() @ k.abs()).masked_fill(late, 0) \
+        .amax(-1, keepdim=True) * abs(scale) + 2.0 ** -20
+    # numerator and denominator each carry a weight's half step of 2^-11 and
+    # twice the error of two scores; the row's largest weight over the sum is
+    # the largest of p. Tokens whose weight fp32 cannot hold add nothing.
+    held = (p > 2.0 ** -140).double()
+    floor = step * p.amax(-1, keepdim=True) * (held @ v.amax(-1, keepdim=True))
+    bound = (size + out.abs().transpose(0, 1)) * (2.0 ** -11 + 4 * ds) + floor
+    return out, bound.transpose(0, 1)
+
+
 def norm_rope(x, w, cos, sin, pos, eps, interleaved):
     """x [B, T, H, hd], pos [B, T] -> (fp64 result, error bound before the
     last rounding)."""
