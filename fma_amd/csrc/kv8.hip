@@ -26,6 +26,7 @@ struct Bf16 {
   typedef uint16_t raw;
   static constexpr uint32_t kInf = 0x7f80, kMaxFinite = 0x7f7f;
   static constexpr float kMost = 3.3895313892515355e38f;
+  static constexpr float kFine = 1.0f;
   static __device__ float to_f(uint16_t u) {
     return __uint_as_float(static_cast<uint32_t>(u) << 16);
   }
@@ -37,6 +38,7 @@ struct Fp16 {
   typedef uint16_t raw;
   static constexpr uint32_t kInf = 0x7c00, kMaxFinite = 0x7bff;
   static constexpr float kMost = 65504.0f;
+  static constexpr float kFine = 16384.0f;  // keeps a second part's bits
   static __device__ float to_f(uint16_t u) {
     return static_cast<float>(__builtin_bit_cast(_Float16, u));
   }
@@ -858,7 +860,7 @@ struct AttnArgs {
   FmaKv8Span sp;
   FmaRows q;
   void* out;
-  float* partials;  // [rows, splits, HDP]
+  float* partials;  // [rows, splits, HDP]: a part's own outputs
   float* stats;     // [rows, splits, 2]: reference and sum
   float scale;  // of the scores, its magnitude times log2(e)
   int negative;
@@ -1086,13 +1088,21 @@ __device__ inline float query_fp16(const AttnArgs& A, const u16x8 (&raw)[NS],
   return A.scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 }
 
-// The incomplete block, raw, for NR times 16 rows. Its weights go in as two
-// 16-bit parts: a single bf16 would cost as much as the result's rounding.
+// What ends a wave's part of NR times 16 rows: the incomplete block, raw, where
+// it reads one, and the division by the sums. Outputs are in units of `unit`
+// before and whole values after; l is then the row's whole sum in each lane.
+// They are divided before the raw values and the parts of a row come together,
+// so that no sum is larger than the largest V, which may be the type's largest
+// (1000 tokens of 3e38 once gave infinity). A code may stand for a little more
+// than that: outputs saturate, and NaN stays.
+// The raw block's weights go in as two 16-bit parts: a single bf16 would cost
+// as much as the result's rounding.
 template <int NS, int NR, typename E, bool FP8>
-__device__ inline void tail_step(const AttnArgs& A, const Reach& R, int bh,
-                                 int lane, const u16x8 (&q)[NR][NS],
-                                 const int (&seen)[NR],
-                                 RowState<NS, FP8> (&st)[NR]) {
+__device__ inline void conclude(const AttnArgs& A, const Reach& R, bool tail,
+                                int bh, int lane,
+                                const uint16_t* const (&qrow)[NR],
+                                const bool (&live)[NR], const int (&seen)[NR],
+                                float unit, RowState<NS, FP8> (&st)[NR]) {
   const int g = lane >> 4;
   const uint16_t* const kt =
       static_cast<const uint16_t*>(A.c.tail) +
@@ -1100,74 +1110,97 @@ __device__ inline void tail_step(const AttnArgs& A, const Reach& R, int bh,
       lane * 16;
   const uint16_t* const vt = kt + A.c.tail_v;
   f32x4 x[1][NR][2];
-  float f[1][NR];
-#pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    x[0][r][0] = x[0][r][1] = f32x4{0, 0, 0, 0};
-    f[0][r] = A.scale;
-  }
-#pragma unroll
-  for (int ks = 0; ks < NS; ++ks)
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      const u16x8 k = *reinterpret_cast<const u16x8*>(kt + ks * 1024 + a * 8);
-#pragma unroll
-      for (int r = 0; r < NR; ++r)
-        x[0][r][a] = mfma16<E>(k, q[r][ks], x[0][r][a]);
-    }
-#pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    if (A.negative) {
-      x[0][r][0] = -x[0][r][0];
-      x[0][r][1] = -x[0][r][1];
-    }
-    mask(x[0][r], seen[r] - R.full * BLK - 4 * g);
-  }
-  settle<NR, 1>(x, f, st, 1.0f);
-  u16x8 hi[NR], lo[NR];
-#pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    weigh<true>(x[0][r], A.scale, st[r]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float p = x[0][r][i >> 2][i & 3];
-      const uint16_t u = E::from_f(p);
-      hi[r][i] = u;
-      lo[r][i] = E::from_f(p - E::to_f(u));
-    }
-  }
-  const int held = R.held - R.full * BLK - 4 * g;
-#pragma unroll
-  for (int n = 0; n < 2 * NS; ++n) {
-    u16x8 v = *reinterpret_cast<const u16x8*>(vt + (n >> 1) * 1024 +
-                                              (n & 1) * 8);
-    const u16x8 m = v & static_cast<uint16_t>(0x7fff);
-    uint32_t most = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) most = max(most, static_cast<uint32_t>(m[i]));
-    if (__builtin_expect(__any(most >= E::kInf), 0)) {
-      // NaN or infinities, in tokens or behind them
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[i] = 16 * (i >> 2) + (i & 3) < held ? tame<E>(v[i]) : 0;
-    }
+  if (tail) {
+    u16x8 q[NR][NS];
+    float f[1][NR];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      st[r].o[n] = mfma16<E>(v, hi[r], st[r].o[n]);
-      st[r].o[n] = mfma16<E>(v, lo[r], st[r].o[n]);
+      load_query<NS, E>(A, qrow[r], live[r], g, q[r]);
+      x[0][r][0] = x[0][r][1] = f32x4{0, 0, 0, 0};
+      f[0][r] = A.scale;
+    }
+#pragma unroll
+    for (int ks = 0; ks < NS; ++ks)
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const u16x8 k = *reinterpret_cast<const u16x8*>(kt + ks * 1024 + a * 8);
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+          x[0][r][a] = mfma16<E>(k, q[r][ks], x[0][r][a]);
+      }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      if (A.negative) {
+        x[0][r][0] = -x[0][r][0];
+        x[0][r][1] = -x[0][r][1];
+      }
+      mask(x[0][r], seen[r] - R.full * BLK - 4 * g);
+    }
+    settle<NR, 1>(x, f, st, 1.0f);
+#pragma unroll
+    for (int r = 0; r < NR; ++r) weigh<true>(x[0][r], A.scale, st[r]);
+  }
+  float by[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    float l = st[r].l;
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    st[r].l = l;
+    by[r] = l == 0.0f ? 0.0f : 1.0f / l;  // nothing seen gives zeros
+    st[r].times(unit * by[r] * (tail ? E::kFine : 1.0f));
+  }
+  if (tail) {
+    u16x8 hi[NR], lo[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float p = x[0][r][i >> 2][i & 3] * by[r] * E::kFine;
+        const uint16_t u = E::from_f(p);
+        hi[r][i] = u;
+        lo[r][i] = E::from_f(p - E::to_f(u));
+      }
+    const int held = R.held - R.full * BLK - 4 * g;
+#pragma unroll
+    for (int n = 0; n < 2 * NS; ++n) {
+      u16x8 v = *reinterpret_cast<const u16x8*>(vt + (n >> 1) * 1024 +
+                                                (n & 1) * 8);
+      const u16x8 m = v & static_cast<uint16_t>(0x7fff);
+      uint32_t most = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = max(most, static_cast<uint32_t>(m[i]));
+      if (__builtin_expect(__any(most >= E::kInf), 0)) {
+        // NaN or infinities, in tokens or behind them
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          v[i] = 16 * (i >> 2) + (i & 3) < held ? tame<E>(v[i]) : 0;
+      }
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        st[r].o[n] = mfma16<E>(v, hi[r], st[r].o[n]);
+        st[r].o[n] = mfma16<E>(v, lo[r], st[r].o[n]);
+        if (E::kFine != 1.0f) st[r].o[n] *= 1.0f / E::kFine;
+      }
     }
   }
+#pragma unroll
+  for (int r = 0; r < NR; ++r)
+#pragma unroll
+    for (int n = 0; n < 2 * NS; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        st[r].o[n][i] = __builtin_elementwise_maximum(
+            __builtin_elementwise_minimum(st[r].o[n][i], E::kMost), -E::kMost);
 }
 
-// Four values of an output row, o / sum; nothing seen gives zeros.
+// Four values of an output row.
 template <typename E>
-__device__ inline void put_row(uint16_t* row, int d, int hd, f32x4 o,
-                               float sum) {
-  const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+__device__ inline void put_row(uint16_t* row, int d, int hd, f32x4 o) {
   typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
   u16x4 u;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) u[i] = E::from_f(o[i] * by);
+  for (int i = 0; i < 4; ++i) u[i] = E::from_f(o[i]);
   if (hd % 4 == 0) {
     if (d < hd) *reinterpret_cast<u16x4*>(row + d) = u;
   } else {
@@ -1289,24 +1322,20 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
       }
       if (!AHEAD && blk + 4 < R.hi) load_v(blk + 4);
     }
-    st.times(vs.ref);
-    if (R.tail && wave == 3) {
-      load_query<NS, E>(A, qrow, live, g, raw[0]);
-      const int sees[1] = {seen};
-      tail_step<NS, 1, E>(A, R, bh, lane, raw, sees, state);
-    }
+    const uint16_t* const rows[1] = {qrow};
+    const bool lives[1] = {live};
+    const int sees[1] = {seen};
+    conclude<NS, 1, E>(A, R, R.tail && wave == 3, bh, lane, rows, lives, sees,
+                       vs.ref, state);
   }
 
   // join the four waves
-  float l = st.l;
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
 #pragma unroll
   for (int n = 0; n < 2 * NS; ++n)
     *reinterpret_cast<f32x4*>(&s_o[wave][n16][16 * n + 4 * g]) = st.o[n];
   if (g == 0) {
     s_m[wave][n16] = st.m;
-    s_l[wave][n16] = l;
+    s_l[wave][n16] = st.l;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 4 * HDP; i += 256) {
@@ -1315,19 +1344,22 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
     if (orow >= A.rows) continue;
     const float m = fmaxf(fmaxf(s_m[0][rr], s_m[1][rr]),
                           fmaxf(s_m[2][rr], s_m[3][rr]));
-    f32x4 o = {0, 0, 0, 0};
-    float sum = 0.0f;
+    float f[4], sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float f = __builtin_amdgcn_exp2f(s_m[w][rr] - m);
-      o += *reinterpret_cast<const f32x4*>(&s_o[w][rr][d]) * f;
-      sum += s_l[w][rr] * f;
+      f[w] = s_l[w][rr] * __builtin_amdgcn_exp2f(s_m[w][rr] - m);
+      sum += f[w];
     }
+    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+    f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      o += *reinterpret_cast<const f32x4*>(&s_o[w][rr][d]) * (f[w] * by);
     const int ot = orow / A.group, oh = h * A.group + (orow - ot * A.group);
     const long long at =
         (static_cast<long long>(b) * A.sp.T + ot) * A.q_heads + oh;
     if (A.splits == 1) {
-      put_row<E>(static_cast<uint16_t*>(A.out) + at * c.hd, d, c.hd, o, sum);
+      put_row<E>(static_cast<uint16_t*>(A.out) + at * c.hd, d, c.hd, o);
     } else {
       *reinterpret_cast<f32x4*>(A.partials + (at * A.splits + split) * HDP +
                                 d) = o;
@@ -1388,6 +1420,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
       last_row / A.group < R.s.count;
   const int clear = whole_wave ? (R.s.start + first + 1) / BLK : 0;
 
+  float unit = 0.0f;
   if (R.lo < R.hi) {
     const unsigned char* const kc =
         c.codes + static_cast<long long>(bh) * c.nblk * BLK * HDP;
@@ -1537,27 +1570,18 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
       step(blk, 0, one, two);
       if (blk + NE < R.hi) step(blk + NE, 1, two, one);
     }
+    unit = vs.ref;
+    if (FP8) {
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      st[r].times(vs.ref);
-      if (FP8) st[r].l *= 0.25f;  // this lane's share again
+      for (int r = 0; r < NR; ++r) st[r].l *= 0.25f;  // a lane's share again
     }
   }
-  if (R.tail) {
-    u16x8 raw[NR][NS];
-#pragma unroll
-    for (int r = 0; r < NR; ++r)
-      load_query<NS, E>(A, qrow[r], live[r], g, raw[r]);
-    tail_step<NS, NR, E>(A, R, bh, lane, raw, seen, st);
-  }
+  conclude<NS, NR, E>(A, R, R.tail, bh, lane, qrow, live, seen, unit, st);
 
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     const int row = tile * ROWS + (wave * NR + r) * 16 + n16;
     if (row >= A.rows) continue;
-    float l = st[r].l;
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
     const int t = row / A.group, hq = h * A.group + (row - t * A.group);
     const long long at =
         (static_cast<long long>(b) * A.sp.T + t) * A.q_heads + hq;
@@ -1565,7 +1589,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
       uint16_t* const out = static_cast<uint16_t*>(A.out) + at * c.hd;
 #pragma unroll
       for (int n = 0; n < 2 * NS; ++n)
-        put_row<E>(out, 16 * n + 4 * g, c.hd, st[r].o[n], l);
+        put_row<E>(out, 16 * n + 4 * g, c.hd, st[r].o[n]);
     } else {
       float* const part = A.partials + (at * A.splits + split) * HDP;
 #pragma unroll
@@ -1574,7 +1598,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
       if (g == 0) {
         float* const s2 = A.stats + (at * A.splits + split) * 2;
         s2[0] = st[r].m;
-        s2[1] = l;
+        s2[1] = st[r].l;
       }
     }
   }
@@ -1592,7 +1616,6 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(const float* partials,
   constexpr int TURNS = (kMaxSplits + GROUPS - 1) / GROUPS;
   __shared__ float s_w[kMaxSplits];
   __shared__ f32x4 s_o[GROUPS][LANES];
-  __shared__ float s_sum;
   const long long row = blockIdx.x;
   const int tid = threadIdx.x, grp = tid / LANES, lane = tid % LANES;
   const float* const p = partials + row * splits * HDP + lane * 4;
@@ -1619,13 +1642,14 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(const float* partials,
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float w = exp2f(m[i] - top);
-      s_w[tid + 64 * i] = w;
-      sum += w * l[i];
+      l[i] *= exp2f(m[i] - top);
+      sum += l[i];
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-    if (tid == 0) s_sum = sum;
+    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) s_w[tid + 64 * i] = l[i] * by;
   }
   __syncthreads();
   if (grp < GROUPS) {
@@ -1646,8 +1670,7 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(const float* partials,
     float o = 0.0f;
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) o += s_o[i][d >> 2][d & 3];
-    const float sum = s_sum;
-    out[row * hd + d] = E::from_f(sum == 0.0f ? 0.0f : o / sum);
+    out[row * hd + d] = E::from_f(o);
   }
 }
 
@@ -1664,15 +1687,15 @@ __global__ __launch_bounds__(256) void kv8_join_rows_kernel(
   const float* const p = partials + row * splits * HDP + d;
   float top = kNone;
   for (int s = 0; s < splits; ++s) top = fmaxf(top, st[2 * s]);
-  f32x4 o = {0, 0, 0, 0};
   float sum = 0.0f;
-  for (int s = 0; s < splits; ++s) {
-    const float w = __builtin_amdgcn_exp2f(st[2 * s] - top);
+  for (int s = 0; s < splits; ++s)
+    sum += __builtin_amdgcn_exp2f(st[2 * s] - top) * st[2 * s + 1];
+  const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+  f32x4 o = {0, 0, 0, 0};
+  for (int s = 0; s < splits; ++s)
     o += *reinterpret_cast<const f32x4*>(p + static_cast<long long>(s) * HDP) *
-         w;
-    sum += w * st[2 * s + 1];
-  }
-  put_row<E>(out + row * hd, d, hd, o, sum);
+         (__builtin_amdgcn_exp2f(st[2 * s] - top) * st[2 * s + 1] * by);
+  put_row<E>(out + row * hd, d, hd, o);
 }
 
 // Heads that a row of lanes takes: as many as leave every CU six workgroups

@@ -11,7 +11,8 @@ The largest magnitude counts as at least 2^-100. A block is coded once, when
 its last token arrives; until then its tokens are held as they came, in 16
 bits. Codes are made from 16-bit values, so what the cache holds does not
 depend on how tokens were spread over calls. In a coded block NaN is 0 and an
-infinity the block's largest value.
+infinity the block's largest value; attention takes a V that is still raw
+alike, an infinity as the type's largest value.
 
 The raw values of the last two blocks stay, so a caller may go back a few
 tokens (a rejected draft) and append again: to any position not before the
@@ -268,7 +269,8 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, layer: int,
     start.. and are in the cache already, over everything up to themselves:
     softmax(scale * q K^T) V, scale = head_dim ** -0.5 by default, qH a
     multiple of kvH. start and counts as in :func:`kv8_append`; rows behind a
-    sequence's count come out as zeros. Where the cache knows its length the
+    sequence's count come out as zeros, and outputs saturate at the type's
+    largest value, as which an infinity in V counts. Where the cache knows its length the
     queries may lie anywhere in it; else, and in a captured graph, each
     sequence's last query has to be the last token stored, which says what of
     it is coded already."""
@@ -437,6 +439,7 @@ def _attend(q: torch.Tensor, cache: KV8Cache, layer: int, start: Position,
     T, group = q.shape[1], q.shape[2] // cache.kv_heads
     starts, ns = _host_span(cache, start, T, counts)
     out = torch.zeros(q.shape, dtype=torch.float32)
+    top = torch.finfo(cache.dtype).max
     for b in range(cache.batch):
         s, n = int(starts[b]), int(ns[b])
         if not n:
@@ -444,9 +447,9 @@ def _attend(q: torch.Tensor, cache: KV8Cache, layer: int, start: Position,
         k, v = (x[:s + n].repeat_interleave(group, 1).transpose(0, 1)
                 for x in _held(cache, layer, b,
                                max(cache._length[layer] or 0, s + n)))
-        v = torch.nan_to_num(v)
+        v = torch.nan_to_num(v, posinf=top, neginf=-top)
         score = q[b, :n].float().transpose(0, 1) @ k.transpose(1, 2) * scale
         late = torch.arange(s + n) > s + torch.arange(n)[:, None]
         p = torch.softmax(score.masked_fill(late, float("-inf")), -1)
         out[b, :n] = (p @ v).transpose(0, 1)
-    return out.to(q.dtype)
+    return out.clamp(-top, top).to(q.dtype)

@@ -927,3 +927,42 @@ def test_attention_first_token_holds_the_rows(ops, fmt, B, T, n, H, group):
         last = (bound[-1] / want[-1].abs()).max()
         assert last < 0.6, last
         oracle.check(out[b], want, bound, BF)
+
+
+# -- V near the largest value of its type --------------------------------------
+
+SHAPES = [(1, 75, 2, 8, 1), (1, 5000, 2, 8, 1), (150, 300, 2, 8, 1),
+          (70, 4000, 2, 12, 1), (200, 3300, 1, 16, 1)]
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("T,n,H,qh,B", SHAPES)
+def test_attention_near_the_largest_values(ops, fmt, T, n, H, qh, B):
+    """Sums of weights times such values fit fp32 only once divided."""
+    c, k, v = filled(ops, n, H=H, B=B, hd=64, fmt=fmt)
+    u = torch.rand(v.shape, generator=torch.Generator("cuda").manual_seed(5),
+                   device="cuda")
+    v = ((0.5 + 0.5 * u) * 3e38).to(BF)
+    ops.kv8_append(c, 1, k, v, 0)
+    q = randn(B, T, qh, 64, seed=2)
+    attend_and_check(ops, c, q, k, v, n - T)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("T,n,H,qh,B", SHAPES)
+def test_attention_saturates(ops, fmt, dtype, T, n, H, qh, B):
+    """Codes of the type's largest value stand for a little more; an infinity
+    that is still raw counts as that value."""
+    most = torch.finfo(dtype).max
+    c, k, v = filled(ops, n, H=H, B=B, hd=64, fmt=fmt, dtype=dtype)
+    v.fill_(most)
+    v[:, :, :, 5] = -most
+    v[:, n // 32 * 32:, :, 7] = float("inf")
+    ops.kv8_append(c, 1, k, v, 0)
+    q = randn(B, T, qh, 64, seed=2, dtype=dtype)
+    out = ops.kv8_attention(q, c, 1, n - T).double()
+    want = torch.full_like(out, most)
+    want[..., 5] = -most
+    # weights and codes are off by at most 2^-8 of what they stand for
+    assert ((out - want).abs() <= 2.0 ** -7 * most).all()

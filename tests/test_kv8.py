@@ -403,3 +403,23 @@ def test_option_does_not_keep_a_model_from_being_served(monkeypatch, capsys):
         assert len(rt.rt.generate_text("hello", 3)) >= 0
     finally:
         rt.close()
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_saturates(fmt, dtype):
+    """Codes of the type's largest value stand for a little more; an infinity
+    that is still raw counts as that value."""
+    most = torch.finfo(dtype).max
+    for T, n in ((1, 75), (20, 40), (3, 3)):
+        k, v = kv(n, dtype=dtype)
+        v.fill_(most)
+        v[..., 5] = -most
+        v[:, n // 32 * 32:, :, 7] = float("inf")
+        c = make(fmt, dtype)
+        kv8_append(c, 0, k, v, 0)
+        out = kv8_attention(torch.randn(1, T, 4, 16).to(dtype), c, 0,
+                            n - T).double()
+        want = torch.full_like(out, most)
+        want[..., 5] = -most
+        assert ((out - want).abs() <= 2.0 ** -7 * most).all()
