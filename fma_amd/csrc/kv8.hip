@@ -893,13 +893,63 @@ __device__ inline float row_max(float x) {
   return fmaxf(x, __shfl_xor(x, 32));
 }
 
-// The running reference of V's scales. It moves where fp16 has no room for
-// the ratio to it; down only as far as fp32 sums cannot overflow. Beside the
-// weights (int8) there is room for a ratio of 2.
+// Blocks whose largest V is under about 2^-99 (zeros): they count as nothing
+// beside others.
+constexpr uint32_t kNothing = (127u - 106u) << 23;
+
+// Whether V's scales of blocks [lo, hi) lie within 2^16 of each other, the same
+// in all lanes. A wave looks at all of its part's before it starts (asked
+// block by block, the kernel for many rows took 4% longer): those of the first
+// 64 blocks are asked for ahead of the codes, and one vote says whether all are
+// within 2^8 of the first, as any model's are; only then minima and maxima.
+struct Scales {
+  const float* at;
+  int lo, hi, lane;
+  uint32_t first, mine;
+  __device__ Scales(const float* vsc, int lo_, int hi_, int lane_)
+      : at(vsc), lo(lo_), hi(hi_), lane(lane_) {
+    first = mine = 0;
+    if (lo < hi) {
+      first = __float_as_uint(at[lo]);
+      mine = __float_as_uint(at[min(lo + lane, hi - 1)]);
+    }
+  }
+  __device__ bool near() const {
+    constexpr uint32_t kSide = 8u << 23;
+    bool odd = first < kNothing;
+    uint32_t u = mine;
+    for (int i = lo; i < hi; i += 64) {
+      if (i > lo) u = __float_as_uint(at[min(i + lane, hi - 1)]);
+      odd |= u >= kNothing && u - first + kSide > 2 * kSide;
+    }
+    if (__builtin_expect(!__any(odd), 1)) return true;
+    uint32_t least = 0x7f800000u, most = 0;
+    for (int i = lo + lane; i < hi; i += 64) {
+      u = __float_as_uint(at[i]);
+      if (u >= kNothing) {
+        least = min(least, u);
+        most = max(most, u);
+      }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      least = min(least, static_cast<uint32_t>(__shfl_xor(least, o)));
+      most = max(most, static_cast<uint32_t>(__shfl_xor(most, o)));
+    }
+    return __builtin_amdgcn_readfirstlane(most == 0 ||
+                                          most - least <= 2 * kSide);
+  }
+};
+
+// The running reference of V's scales, of which a wave's outputs are
+// multiples. It moves where fp16 has no room for the ratio to it (beside the
+// weights, int8, there is room for a ratio of 2), and so follows blocks that
+// some rows, or all, give no weight, or do not see. Within 2^16 that loses
+// nothing; where scales lie further apart far_steps does without it.
 template <bool FP8>
 struct ScaleRef {
   static constexpr uint32_t kUp = FP8 ? 6 : 1;
-  float ref = 0.0f, inv = 0.0f, most = 0.0f;
+  float ref = 0.0f, inv = 0.0f;
   // a difference of bits is one of exponents, to a part of one
   __device__ bool far(float scale) const {
     return static_cast<uint32_t>(__float_as_int(scale) - __float_as_int(ref) +
@@ -907,12 +957,11 @@ struct ScaleRef {
   }
   // moves it where need be; returns what to multiply outputs with
   __device__ float follow(float scale) {
-    if (!far(scale) || (scale < ref && !(scale >= most * 5.4e-20f)))
+    if (!far(scale) || (ref != 0.0f && __float_as_uint(scale) < kNothing))
       return 1.0f;
     const float f = ref != 0.0f ? ref / scale : 1.0f;
     ref = scale;
     inv = 1.0f / scale;
-    most = fmaxf(most, scale);
     return f;
   }
   // scale / ref; between powers of two it is a difference of exponents
@@ -1088,9 +1137,94 @@ __device__ inline float query_fp16(const AttnArgs& A, const u16x8 (&raw)[NS],
   return A.scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 }
 
+// Blocks blk, blk + by, .. for NR times 16 rows of a wave, where V's scales lie
+// further apart than one reference serves: a row's outputs are in units of
+// its own, unit[r] * kFarUnit, the largest product of a weight and a scale so
+// far. So neither a block that it gives no weight nor one that it does not see
+// moves them, and each block's weights are rounded against its own largest.
+// Any order of magnitudes of V comes out (weights under 2^-110 are dropped);
+// no real model's V gets here, and a block takes two to three times as long.
+constexpr float kFarUnit = 65536.0f;
+template <int NS, int NR, bool FP8>
+__device__ inline void far_steps(const unsigned char* kc,
+                                 const unsigned char* vc, const float* ksc,
+                                 const float* vsc, int lane, int blk, int hi,
+                                 int by, const int (&seen)[NR],
+                                 const h8 (&q)[NR][NS],
+                                 const float (&qscale)[NR],
+                                 RowState<NS, FP8> (&st)[NR],
+                                 float (&unit)[NR]) {
+  using RS = RowState<NS, FP8>;
+  constexpr float kTop = 16384.0f;  // a block's largest weight in fp16
+  const int g = lane >> 4;
+  for (; blk < hi; blk += by) {
+    const long long at = static_cast<long long>(blk) * BLK * NS * 32 + lane * 16;
+    const float kscale = ksc[blk], vscale = vsc[blk] * (1.0f / kFarUnit);
+    f32x4 x[NR][2];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) x[r][0] = x[r][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int ks = 0; ks < NS; ++ks) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(kc + at + ks * 1024);
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const h8 kf = decode8(w[2 * a], w[2 * a + 1], 1.0f, FP8);
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+          x[r][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[r][ks],
+                                                           x[r][a], 0, 0, 0);
+      }
+    }
+    h8 p[NR];
+    float with[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const float f = factor(kscale, qscale[r]);
+      mask(x[r], seen[r] - blk * BLK - 4 * g);
+      float top = x[r][0][0], most = 0.0f;
+#pragma unroll
+      for (int i = 1; i < 8; ++i) top = fmaxf(top, x[r][i >> 2][i & 3]);
+      top = row_max(top * f);
+      const float next = top > st[r].m + RS::MOST ? top - RS::LEAD : st[r].m;
+      const float less = exp2f(st[r].m - next);
+      st[r].m = next;
+      st[r].l *= less;
+      unit[r] *= less;
+      weigh<true>(x[r], f, st[r]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, x[r][i >> 2][i & 3]);
+      most = row_max(most);
+      const bool any = most > 7.7e-34f;
+      const float mine = any ? most * vscale : 0.0f;
+      const float now = fmaxf(unit[r], mine);
+      with[r] = now > 0.0f ? mine / now * (1.0f / kTop) : 0.0f;
+      st[r].times(now > 0.0f ? unit[r] / now : 1.0f);
+      unit[r] = now;
+      const float to = any ? kTop / most : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        p[r][i] = static_cast<_Float16>(x[r][i >> 2][i & 3] * to);
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(vc + at + i * 1024);
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const h8 vf = decode8(w[2 * a], w[2 * a + 1], 1.0f, FP8);
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+          st[r].o[2 * i + a] +=
+              __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  vf, p[r], f32x4{0, 0, 0, 0}, 0, 0, 0) * with[r];
+      }
+    }
+  }
+}
+
 // What ends a wave's part of NR times 16 rows: the incomplete block, raw, where
-// it reads one, and the division by the sums. Outputs are in units of `unit`
-// before and whole values after; l is then the row's whole sum in each lane.
+// it reads one, and the division by the sums. Outputs are in units of
+// unit[r] * more before and whole values after; l is then the row's whole sum
+// in each lane.
 // They are divided before the raw values and the parts of a row come together,
 // so that no sum is larger than the largest V, which may be the type's largest
 // (1000 tokens of 3e38 once gave infinity). A code may stand for a little more
@@ -1102,7 +1236,8 @@ __device__ inline void conclude(const AttnArgs& A, const Reach& R, bool tail,
                                 int bh, int lane,
                                 const uint16_t* const (&qrow)[NR],
                                 const bool (&live)[NR], const int (&seen)[NR],
-                                float unit, RowState<NS, FP8> (&st)[NR]) {
+                                const float (&unit)[NR], float more,
+                                RowState<NS, FP8> (&st)[NR]) {
   const int g = lane >> 4;
   const uint16_t* const kt =
       static_cast<const uint16_t*>(A.c.tail) +
@@ -1148,7 +1283,8 @@ __device__ inline void conclude(const AttnArgs& A, const Reach& R, bool tail,
     l += __shfl_xor(l, 32);
     st[r].l = l;
     by[r] = l == 0.0f ? 0.0f : 1.0f / l;  // nothing seen gives zeros
-    st[r].times(unit * by[r] * (tail ? E::kFine : 1.0f));
+    // (by times more first: unit alone may be near fp32's largest)
+    st[r].times(unit[r] * (by[r] * more) * (tail ? E::kFine : 1.0f));
   }
   if (tail) {
     u16x8 hi[NR], lo[NR];
@@ -1275,6 +1411,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
         vr[i] = get<PAST, u32x4>(vc + at + i * 1024);
       v_next = vsc[blk];
     };
+    const Scales scales(vsc, R.lo, R.hi, lane);
     int blk = R.lo + wave;
     if (blk < R.hi) {
       load_k(blk);
@@ -1283,10 +1420,14 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
     const uint16_t* const qrow = static_cast<const uint16_t*>(A.q.p) +
                                  b * A.q.sb + t * A.q.st + hq * A.q.sh;
     u16x8 raw[1][NS];
-    h8 q[NS];
+    h8 qs[1][NS];
+    h8(&q)[NS] = qs[0];
     load_query<NS, E>(A, qrow, live, g, raw[0]);
     const float qscale = query_fp16<NS, E>(A, raw[0], q);
-    for (; blk < R.hi; blk += 4) {
+    const int sees[1] = {seen};
+    const bool near = scales.near();
+    const int end = near ? R.hi : R.lo;
+    for (; blk < end; blk += 4) {
       const float kscale = k_next;
       f32x4 xs[1][1][2] = {{{{0, 0, 0, 0}, {0, 0, 0, 0}}}};
       f32x4(&x)[2] = xs[0][0];
@@ -1324,9 +1465,15 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
     }
     const uint16_t* const rows[1] = {qrow};
     const bool lives[1] = {live};
-    const int sees[1] = {seen};
+    float unit[1] = {vs.ref}, more = 1.0f;
+    if (__builtin_expect(!near, 0)) {
+      more = kFarUnit;
+      const float qscales[1] = {qscale};
+      far_steps<NS, 1>(kc - lane * 16, vc - lane * 16, ksc, vsc, lane, blk,
+                       R.hi, 4, sees, qs, qscales, state, unit);
+    }
     conclude<NS, 1, E>(A, R, R.tail && wave == 3, bh, lane, rows, lives, sees,
-                       vs.ref, state);
+                       unit, more, state);
   }
 
   // join the four waves
@@ -1384,8 +1531,12 @@ template <int NS, bool FP8, typename E, int NR, int NE>
 __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
   constexpr int HDP = NS * 32;
   constexpr int UNITS = NS * 64;  // of 16 codes in a block of K or V
-  // a lane's operand of each 32 by 16 values, by lanes
-  __shared__ h8 s_k[2][NE][2 * NS][64], s_v[2][NE][2 * NS][64];
+  // a lane's operand of each 32 by 16 values, by lanes. At a width of 192 the
+  // compiler would save registers for a third workgroup on a CU, which costs
+  // more than it gives (int8, 4 x 512 tokens behind 2000: 196 us against 165
+  // us); 8 KB more say that none fits.
+  constexpr int ROOM = NS == 6 ? 2 : 0;
+  __shared__ h8 s_k[2][NE][2 * NS + ROOM][64], s_v[2][NE][2 * NS + ROOM][64];
   const FmaKv8Layer& c = A.c;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g = lane >> 4, n16 = lane & 15;
@@ -1420,7 +1571,9 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
       last_row / A.group < R.s.count;
   const int clear = whole_wave ? (R.s.start + first + 1) / BLK : 0;
 
-  float unit = 0.0f;
+  float unit[NR], unit_by = 1.0f;
+#pragma unroll
+  for (int r = 0; r < NR; ++r) unit[r] = 0.0f;
   if (R.lo < R.hi) {
     const unsigned char* const kc =
         c.codes + static_cast<long long>(bh) * c.nblk * BLK * HDP;
@@ -1452,6 +1605,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
       if (lane < 2 * NE)
         to.scale = (lane < NE ? ksc : vsc)[min(blk + lane % NE, R.hi - 1)];
     };
+    const Scales scales(vsc, R.lo, R.hi, lane);
     Staged one, two;
     one.scale = two.scale = 0.0f;
     load(one, R.lo);
@@ -1499,6 +1653,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
         }
       }
     };
+    const bool near = scales.near();
     store(one, 0);
     __syncthreads();
     // the blocks in LDS; `later` is filled with those after the next
@@ -1566,17 +1721,24 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
       __builtin_amdgcn_s_setprio(0);
       __syncthreads();
     };
-    for (int blk = R.lo; blk < R.hi; blk += 2 * NE) {
-      step(blk, 0, one, two);
-      if (blk + NE < R.hi) step(blk + NE, 1, two, one);
-    }
-    unit = vs.ref;
-    if (FP8) {
+    if (near) {
+      for (int blk = R.lo; blk < R.hi; blk += 2 * NE) {
+        step(blk, 0, one, two);
+        if (blk + NE < R.hi) step(blk + NE, 1, two, one);
+      }
 #pragma unroll
-      for (int r = 0; r < NR; ++r) st[r].l *= 0.25f;  // a lane's share again
+      for (int r = 0; r < NR; ++r) {
+        unit[r] = vs.ref;
+        if (FP8) st[r].l *= 0.25f;  // this lane's share again
+      }
+    } else {
+      unit_by = kFarUnit;
+      far_steps<NS, NR>(kc, vc, ksc, vsc, lane, R.lo, R.hi, 1, seen, q, qscale,
+                        st, unit);
     }
   }
-  conclude<NS, NR, E>(A, R, R.tail, bh, lane, qrow, live, seen, unit, st);
+  conclude<NS, NR, E>(A, R, R.tail, bh, lane, qrow, live, seen, unit, unit_by,
+                      st);
 
 #pragma unroll
   for (int r = 0; r < NR; ++r) {

@@ -966,3 +966,73 @@ def test_attention_saturates(ops, fmt, dtype, T, n, H, qh, B):
     want[..., 5] = -most
     # weights and codes are off by at most 2^-8 of what they stand for
     assert ((out - want).abs() <= 2.0 ** -7 * most).all()
+
+
+# -- blocks of V that lie any number of magnitudes apart -----------------------
+
+def one_block_each(n, T, H, qh, hd, span, seed=0):
+    """Keys of block j point along axis j, each query row along that of a
+    block that it sees, 2^200 above the others; V's blocks lie `span` (log2)
+    apart."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def rand(*shape):
+        return torch.randn(*shape, generator=g, device="cuda")
+    blocks = (n + 31) // 32
+    side = (200 * 0.6931 * hd ** 0.5) ** 0.5
+    k = 0.02 * rand(1, n, H, hd)
+    at = torch.arange(n, device="cuda") // 32
+    k[:, torch.arange(n, device="cuda"), :, at] += side
+    up = torch.rand(blocks, generator=g, device="cuda") \
+        * (span[1] - span[0]) + span[0]
+    up[0], up[-2] = span[0], span[1]            # the ends among them
+    v = (1 + 0.3 * rand(1, n, H, hd)) * torch.exp2(up[at])[:, None, None]
+    last = (n - T + torch.arange(T, device="cuda")) // 32
+    pick = (torch.rand(T, qh, generator=g, device="cuda")
+            * (last[:, None] + 1)).long()
+    q = 0.02 * rand(1, T, qh, hd)
+    q[0].scatter_add_(2, pick[:, :, None],
+                      torch.full((T, qh, 1), side, device="cuda"))
+    return q.to(BF), k.to(BF), v.to(BF)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("n,T,H,qh,hd", [(20 * 32 + 7, 1, 1, 16, 64),
+                                         (20 * 32 + 7, 40, 2, 16, 64),
+                                         (647, 647, 1, 2, 64),
+                                         (6 * 32 + 1, 193, 1, 3, 32),
+                                         (20 * 32, 3, 2, 8, 256),
+                                         (660, 200, 1, 8, 160)])
+@pytest.mark.parametrize("span", [(-60, 110), (110, -60), (-20, -2),
+                                  (-5, 30)])
+def test_attention_over_blocks_of_any_scale(ops, fmt, n, T, H, qh, hd, span):
+    """A row gives what its own block gives, whatever blocks that it gives no
+    weight, or that come behind it, hold."""
+    q, k, v = one_block_each(n, T, H, qh, hd, span)
+    c = ops.KV8Cache(2, 1, n, H, hd, fmt=fmt, device="cuda")
+    ops.kv8_append(c, 1, k, v, 0)
+    out = ops.kv8_attention(q, c, 1, n - T)
+    want, bound = oracle.attention_tight(
+        q[0], oracle.held(k[0], fmt), oracle.held(v[0], fmt), n - T,
+        hd ** -0.5, 2.0 ** -30)
+    assert (bound < 0.02 * want.abs().amax(-1, keepdim=True)).all()
+    oracle.check(out[0], want, bound, BF)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("T,qh", [(60, 1), (60, 8)])
+def test_attention_does_not_see_later_blocks_of_any_scale(ops, fmt, T, qh):
+    """Values behind a row, finite and huge, in codes and raw."""
+    n, lo = 110, 50
+    c, k, v = filled(ops, n, H=1, fmt=fmt)
+    q = randn(1, T, qh, 128, seed=2)
+    for at in (64, 96):
+        vv = v.clone()
+        vv[:, at:] *= 2.0 ** 120
+        ops.kv8_append(c, 1, k, vv, 0)
+        out = ops.kv8_attention(q, c, 1, lo)
+        want, bound = oracle.attention_tight(
+            q[0], oracle.held(k[0], fmt), oracle.held(vv[0], fmt), lo,
+            128 ** -0.5, 2.0 ** -30)
+        assert (bound[:at - lo] < 0.05).all()
+        oracle.check(out[0], want, bound, BF)
