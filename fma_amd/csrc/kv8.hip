@@ -1124,9 +1124,10 @@ __device__ inline float query_fp16(const AttnArgs& A, const u16x8 (&raw)[NS],
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(E::to_f(raw[ks][i])));
   top = row_max(top);
-  // 2^-e brings the row's largest into [2^9, 2^10)
+  // 2^-e brings the row's largest into [2^9, 2^10), or as near as 2^e is a
+  // normal number: also where it is bf16's largest or smallest
   int e = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 9;
-  e = top == 0.0f ? 0 : min(max(e, -100), 100);
+  e = top == 0.0f ? 0 : max(e, -126);
   const float size = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
   const float mul = A.negative ? -size : size;
 #pragma unroll

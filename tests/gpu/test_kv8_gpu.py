@@ -1036,3 +1036,15 @@ def test_attention_does_not_see_later_blocks_of_any_scale(ops, fmt, T, qh):
             128 ** -0.5, 2.0 ** -30)
         assert (bound[:at - lo] < 0.05).all()
         oracle.check(out[0], want, bound, BF)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("T,n,H,qh,B", SHAPES[:4])
+@pytest.mark.parametrize("qe,ke", [(122, -80), (-118, 100)])
+def test_attention_of_queries_near_the_ends_of_the_type(ops, fmt, T, n, H, qh,
+                                                        B, qe, ke):
+    c, k, v = filled(ops, n, H=H, B=B, hd=64, fmt=fmt)
+    k = (randn(B, n, H, 64, dtype=FP, seed=4) * 2.0 ** ke).to(BF)
+    ops.kv8_append(c, 1, k, v, 0)
+    q = (randn(B, T, qh, 64, dtype=FP, seed=2) * 2.0 ** qe).to(BF)
+    attend_and_check(ops, c, q, k, v, n - T, scale=0.125 * 2.0 ** -(qe + ke))
