@@ -18,6 +18,10 @@ namespace {
 #define KV8_HIP_CHECK(expr)                                             \
   do {                                                                  \
     hipError_t _e = (expr);                                             \
+    /* reported here, not by the next call as well */                   \
+    if (_e != hipSuccess) (void)hipGetLastError();                      \
+    TORCH_CHECK_VALUE(_e != hipErrorInvalidValue,                       \
+                      "sizes beyond one launch, in `" #expr "`");       \
     TORCH_CHECK(_e == hipSuccess, "HIP error — ", hipGetErrorString(_e), \
                 " in `" #expr "`");                                     \
   } while (0)

@@ -1883,9 +1883,12 @@ long long token_groups(long long tokens, int items, int hd) {
   return (units + rows - 1) / rows;
 }
 
+// A launch takes fewer than 2^32 threads in x.
 template <typename... P, typename... Given>
 hipError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t lds,
                   hipStream_t stream, Given... given) {
+  if (static_cast<long long>(grid.x) * threads > 0xffffffffLL)
+    return hipErrorInvalidValue;
   return [&](P... args) {
     void* list[] = {&args...};
     return hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid,

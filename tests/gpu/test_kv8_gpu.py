@@ -1048,3 +1048,17 @@ def test_attention_of_queries_near_the_ends_of_the_type(ops, fmt, T, n, H, qh,
     ops.kv8_append(c, 1, k, v, 0)
     q = (randn(B, T, qh, 64, dtype=FP, seed=2) * 2.0 ** qe).to(BF)
     attend_and_check(ops, c, q, k, v, n - T, scale=0.125 * 2.0 ** -(qe + ke))
+
+
+def test_calls_beyond_one_launch_are_refused(ops):
+    """2^32 threads; nothing is launched, and the next call is not blamed."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 34 GB for the outputs")
+    q = torch.ones(1, 1, 32, 2, dtype=BF, device="cuda") \
+        .expand(1, 1 << 27, 32, 2)
+    cos, sin = oracle.tables(4, 2, "cuda")
+    for _ in range(2):
+        with pytest.raises(ValueError, match="beyond one launch"):
+            ops.fast_qk_norm_rope(q, q, cos, sin, ints(0))
+        assert (torch.ones(1000, device="cuda") * 2).sum().item() == 2000
+    torch.cuda.empty_cache()
