@@ -1062,3 +1062,18 @@ def test_calls_beyond_one_launch_are_refused(ops):
             ops.fast_qk_norm_rope(q, q, cos, sin, ints(0))
         assert (torch.ones(1000, device="cuda") * 2).sum().item() == 2000
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("hd", [16, 32])
+@pytest.mark.parametrize("B,T,n,H,qh", [(1, 300, 301, 2, 12),
+                                        (1, 70, 4000, 2, 12),
+                                        (1, 150, 3300, 1, 16),
+                                        (1, 1, 5000, 2, 8),
+                                        (32, 1, 1500, 2, 64)])
+def test_attention_narrow_heads(ops, fmt, hd, B, T, n, H, qh):
+    """Many rows and both joins (under 2048 rows and from there on) at a
+    width of 32, where one wave of four stages a block."""
+    c, k, v = filled(ops, n, H=H, B=B, hd=hd, fmt=fmt)
+    q = randn(B, T, qh, hd, seed=2)
+    attend_and_check(ops, c, q, k, v, n - T)
