@@ -823,14 +823,20 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(
 //
 // K and V are made fp16 on the way into the matrix unit: e4m3 and int8 fit
 // exactly. A query row is scaled by a power of two to fit fp16, exactly but
-// for values 2^24 below the row's largest. The weights are rounded to fp16:
-// half a step is 2^-11 of each, against 2^-8 of a bf16 result and as much as
-// an fp16 result's own, where a row has no more than a few tokens for it to
-// even out over. So that this holds for small weights too, a row's largest
-// stands at 2^7 or more (int8: 2^6): down to 2^-21 (2^-20) of the largest a
-// weight has all of its bits, and below it is off by at most 2^-32 (2^-31) of
-// the largest. With the largest at 1, 16384 tokens of 2^-26 beside one that
-// holds the row, which first tokens of real models do, all came out as zero.
+// for values 2^24 below the row's largest. The weights go in as fp16. The
+// kernel for few rows waits for memory and has room for two parts of each, 20
+// bits: what comes out is the plain form's but for fp32 rounding (131000 tokens
+// of 4 kv heads 28.3 against 27.9 us with one part, 12 tokens behind 4000 12.1
+// against 11.8 us). The one for many rows takes one, half a step of which is
+// 2^-11 of a weight: against 2^-8 of a bf16 result, and as much as an fp16
+// result's own where a row has no more than a few tokens for it to even out
+// over. Two would cost it a third (2048 tokens behind 6144: 575 against 428
+// us). So that this holds for small weights too, a row's largest stands at
+// 2^8 or more (int8: 2^7): down to 2^-22 (2^-21) of the largest a weight has
+// all of these bits, and below it is off by at most 2^-33 (2^-32) of the
+// largest, twice that where it is cut off.
+// With the largest at 1, 16384 tokens of 2^-26 beside one that holds the row,
+// which first tokens of real models do, all came out as zero.
 // A block's K scale multiplies its scores; its V scale relative to a running
 // reference goes into V's conversion (fp8: a power of two, exact) or the
 // weights (int8).
@@ -984,7 +990,7 @@ constexpr float kNone = -3e38f;
 // beside them.
 template <int NS, bool FP8>
 struct RowState {
-  static constexpr float LEAD = FP8 ? 7.0f : 6.0f, MOST = LEAD + 8.0f;
+  static constexpr float LEAD = FP8 ? 8.0f : 7.0f, MOST = LEAD + 7.0f;
   f32x4 o[2 * NS];  // O^T in units of vref: value 16 n + 4 g + reg, row l % 16
   float m, l;       // running reference and this lane's share of the sum
   __device__ void clear() {
@@ -1010,7 +1016,7 @@ struct RowState {
 };
 
 // x: products of NE blocks with NR times 16 rows; f > 0: what makes them log2
-// scores. A row's reference moves only when a score has grown by 2^8, which
+// scores. A row's reference moves only when a score has grown by 2^7, which
 // fp16 weights and fp32 sums have room for: the outputs are rarely rescaled,
 // and while no lane asks for it, no value has to cross lanes.
 // more: what the outputs are to be multiplied with in any case.
@@ -1075,6 +1081,30 @@ __device__ inline h8 weights16(const f32x4 (&x)[2], float ratio) {
     for (int i = 0; i < 4; ++i)
       p[4 * a + i] = static_cast<_Float16>(FP8 ? x[a][i] : x[a][i] * ratio);
   return p;
+}
+
+// The weights in two fp16 parts, 20 bits of them: both cut off, which is one
+// instruction for two, for the second has what the first leaves.
+template <bool FP8>
+__device__ inline void weights32(const f32x4 (&x)[2], float ratio, h8* p,
+                                 h8* rest) {
+  u32x4 hi, lo;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float w[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      w[j] = x[i >> 1][2 * (i & 1) + j];
+      if (!FP8) w[j] *= ratio;
+    }
+    const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(w[0], w[1]));
+    hi[i] = __builtin_bit_cast(uint32_t, h);
+    lo[i] = __builtin_bit_cast(
+        uint32_t, __builtin_amdgcn_cvt_pkrtz(w[0] - static_cast<float>(h[0]),
+                                             w[1] - static_cast<float>(h[1])));
+  }
+  *p = __builtin_bit_cast(h8, hi);
+  *rest = __builtin_bit_cast(h8, lo);
 }
 
 // Where a tile of query rows reads its keys: its span, the tokens stored, the
@@ -1362,8 +1392,15 @@ __device__ inline V get(const void* at) {
   else
     return *static_cast<const V*>(at);
 }
+// Workgroups a CU: as many as the registers of one part of a weight left; the
+// second would take one off at widths of 64 and 96 (int8, 96: 72.7 against 68.3
+// us for 32 sequences of 8192 tokens).
 template <int NS, bool FP8, typename E, bool PAST>
-__global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(AttnArgs A) {
+__global__ __launch_bounds__(256, NS == 1   ? 6
+                                  : NS == 2 ? (FP8 ? 5 : 4)
+                                  : NS == 3 ? 4
+                                  : NS == 4 ? 3
+                                            : 2) void kv8_attn_few_kernel(AttnArgs A) {
   constexpr int HDP = NS * 32;
   __shared__ alignas(16) float s_o[4][16][HDP + 4];
   __shared__ float s_m[4][16], s_l[4][16];
@@ -1452,15 +1489,17 @@ __global__ __launch_bounds__(256, NS <= 4 ? 3 : 2) void kv8_attn_few_kernel(Attn
       settle<1, 1>(xs, f, state, vs.follow(vscale));
       weigh<true>(x, f[0][0], st);
       const float ratio = vs.ratio(vscale);
-      const h8 p = weights16<FP8>(x, ratio);
+      h8 p, rest;
+      weights32<FP8>(x, ratio, &p, &rest);
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        st.o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-            decode8(v_now[i][0], v_now[i][1], ratio, FP8), p, st.o[2 * i], 0, 0,
-            0);
-        st.o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-            decode8(v_now[i][2], v_now[i][3], ratio, FP8), p, st.o[2 * i + 1],
-            0, 0, 0);
+      for (int i = 0; i < 2 * NS; ++i) {
+        const int a = 2 * (i & 1);
+        const h8 vf = decode8(v_now[i >> 1][a], v_now[i >> 1][a + 1], ratio,
+                              FP8);
+        st.o[i] =
+            __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p, st.o[i], 0, 0, 0);
+        st.o[i] =
+            __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, rest, st.o[i], 0, 0, 0);
       }
       if (!AHEAD && blk + 4 < R.hi) load_v(blk + 4);
     }

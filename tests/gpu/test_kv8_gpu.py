@@ -1077,3 +1077,20 @@ def test_attention_narrow_heads(ops, fmt, hd, B, T, n, H, qh):
     c, k, v = filled(ops, n, H=H, B=B, hd=hd, fmt=fmt)
     q = randn(B, T, qh, hd, seed=2)
     attend_and_check(ops, c, q, k, v, n - T)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("B,T,n", [(4, 1, 75), (4, 1, 700), (2, 1, 5000),
+                                   (2, 12, 800)])
+def test_attention_of_few_rows_holds_20_bits_of_a_weight(ops, fmt, B, T, n):
+    """Two cut-off parts leave less than 2^-10 of 2^-10 of a weight, the
+    rounded ones of the raw block less than that."""
+    hd, H, qh = 32, 2, 8
+    c, k, v = filled(ops, n, H=H, hd=hd, B=B, fmt=fmt, dtype=HF, kscale=0.5)
+    q = randn(B, T, qh, hd, seed=2, dtype=HF, scale=0.5)
+    out = ops.kv8_attention(q, c, 1, n - T)
+    for b in range(B):
+        want, bound = oracle.attention_tight(
+            q[b], oracle.held(k[b], fmt), oracle.held(v[b], fmt), n - T,
+            hd ** -0.5, 2.0 ** -30, 2.0 ** -20)
+        oracle.check(out[b], want, bound, HF)

@@ -69,7 +69,7 @@ def attention(q, k, v, start, scale):
     return out.transpose(0, 1), bound.transpose(0, 1)
 
 
-def attention_tight(q, k, v, start, scale, step):
+def attention_tight(q, k, v, start, scale, step, weight=2.0 ** -11):
     """As :func:`attention`, with a bound that knows that a weight under
     2^-20 of the row's largest is off by at most `step` of it: for each token
     that the row sees, times that token's own largest value (the cache's
@@ -88,12 +88,12 @@ def attention_tight(q, k, v, start, scale, step):
     size = p @ v
     ds = 2.0 ** -24 * q.shape[2] * (qt.abs() @ k.abs()).masked_fill(late, 0) \
         .amax(-1, keepdim=True) * abs(scale) + 2.0 ** -20
-    # numerator and denominator each carry a weight's half step of 2^-11 and
+    # numerator and denominator each carry a weight's own error and
     # twice the error of two scores; the row's largest weight over the sum is
     # the largest of p. Tokens whose weight fp32 cannot hold add nothing.
     held = (p > 2.0 ** -140).double()
     floor = step * p.amax(-1, keepdim=True) * (held @ v.amax(-1, keepdim=True))
-    bound = (size + out.abs().transpose(0, 1)) * (2.0 ** -11 + 4 * ds) + floor
+    bound = (size + out.abs().transpose(0, 1)) * (weight + 4 * ds) + floor
     return out, bound.transpose(0, 1)
 
 
