@@ -1381,7 +1381,7 @@ __device__ inline void put_row(uint16_t* row, int d, int hd, f32x4 o) {
 // each straight from memory into the matrix unit's operands, the next block
 // on its way meanwhile. Bound by memory: 32 sequences of up to 8192 tokens, 8
 // kv heads (270 MB), 54 us with the join, 5.0 TB/s; 131000 tokens of 4 kv
-// heads in int8 27.5 us, 4.9 TB/s. On the vector unit 8 query heads a kv head
+// heads in int8 28.3 us, 4.7 TB/s. On the vector unit 8 query heads a kv head
 // would need more than it has: 13 codes a clock and CU arrive at 8 TB/s.
 // PAST: codes that no cache would keep until they are read again are not put
 // there (270 MB: 58 us against 67 us).
@@ -1564,9 +1564,12 @@ __global__ __launch_bounds__(256, NS == 1   ? 6
 // is decoded once for all of them; the next ones are on their way meanwhile.
 // Bound by what a SIMD can issue: for each 16 products a weight costs an
 // exponential and about ten other vector operations. 2048 tokens behind 6144,
-// 64/8 heads of 128: 431 us, 1.12 PFLOP/s (a large bf16 product: 1.25). Each
-// wave decoding for itself took 511 us, one block at a time 5% more than two,
-// 48 or 64 rows a wave (one wave a SIMD) half as long again.
+// 64/8 heads of 128: 1.04e6 cycles, which is 428 to 475 us on different cards
+// once the clock is up (2.2 to 2.4 GHz, after some 50 calls), 490 to 660 us
+// before (2.0 GHz): 1.12 to 1.01 PFLOP/s, where a large bf16 product reaches
+// 1.25. On one card each wave decoding for itself took 511 us against 495, one
+// block at a time 5% more than two, 48 or 64 rows a wave (one wave a SIMD) half
+// as long again.
 template <int NS, bool FP8, typename E, int NR, int NE>
 __global__ __launch_bounds__(256, 2) void kv8_attn_many_kernel(AttnArgs A) {
   constexpr int HDP = NS * 32;
